@@ -75,6 +75,15 @@ template <typename T> struct alignas(16) Vec16 {
     T v[N];
 };
 
+// The same 16 bytes, opaque to the compiler: it would widen loaded bf16 values where they are loaded and keep them, twice as
+// large, in registers until their use (32 to 64 more registers in the convolution epilogues, spills in the widest).
+template <typename T> __device__ __forceinline__ Vec16<T> as_loaded(Vec16<T> v) {
+    typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+    u4 w = __builtin_bit_cast(u4, v);
+    asm("" : "+v"(w));
+    return __builtin_bit_cast(Vec16<T>, w);
+}
+
 __device__ __forceinline__ float leaky(float z, float slope) { return z > 0.f ? z : z * slope; }
 
 __device__ __forceinline__ float wave_sum(float v) {

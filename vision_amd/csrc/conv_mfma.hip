@@ -977,8 +977,11 @@ conv_ntw_mfma_kernel(Gather gp, const T* __restrict__ x, const T* __restrict__ w
     // the MFMAs of the previous half run, so the eight lock-stepped waves never wait on LDS with
     // the matrix pipe idle.  One barrier per K-step, in its middle: before it a wave has waited for
     // its own loads of the next stage, after it the first half of that stage may be read.
+    // fp32: one set, each half read right before its MFMAs (four times the MFMAs per fragment hide the latency).  With two sets
+    // next to the statistics' sums the kernel spilled 70 registers, and the compiler lost some of the sums among them.
+    constexpr bool TWO_SETS = sizeof(T) == 2;
     Frag a0[4], b0[NT], a1[4], b1[NT];
-    read_frags(0, 0, a0, b0);
+    if constexpr (TWO_SETS) read_frags(0, 0, a0, b0);
     int buf = 0;
     bool stores_behind = false;                            // the previous K-step ended with a tile's NSTORE buffer stores
     for (;;) {
@@ -987,13 +990,15 @@ conv_ntw_mfma_kernel(Gather gp, const T* __restrict__ x, const T* __restrict__ w
             const int nbuf = buf == 2 ? 0 : buf + 1;
             const bool issue = s_more;
             const bool last = k == nk - 1;
-            read_frags(buf, 1, a1, b1);
+            if constexpr (TWO_SETS) read_frags(buf, 1, a1, b1);
+            else read_frags(buf, 0, a0, b0);
 #if VAMD_ABLATE == 10       // timing only: pixel loads for the first tap alone, as if a halo tile served the other eight
             if (issue && tap == 0) stage_a(sbuf);
 #elif VAMD_ABLATE != 4
             if (issue) stage_a(sbuf);
 #endif
             mma(a0, b0);
+            if constexpr (!TWO_SETS) read_frags(buf, 1, a1, b1);
             // the stage read next was issued during the previous K-step: only this K-step's
             // pixel loads may stay in flight; every LDS read issued so far has long returned
 #if VAMD_ABLATE == 1 || VAMD_ABLATE == 3
@@ -1009,7 +1014,9 @@ conv_ntw_mfma_kernel(Gather gp, const T* __restrict__ x, const T* __restrict__ w
 #if VAMD_ABLATE != 2 && VAMD_ABLATE != 3
             __builtin_amdgcn_s_barrier();
 #endif
-            if (!last || cur + rstep < row_tiles) read_frags(nbuf, 0, a0, b0);
+            if constexpr (TWO_SETS) {
+                if (!last || cur + rstep < row_tiles) read_frags(nbuf, 0, a0, b0);
+            }
             if (issue) {
 #if VAMD_ABLATE != 4
                 stage_b(sbuf);
@@ -1320,12 +1327,14 @@ conv_c64_halo_kernel(HaloArgs ha, const bf16_t* __restrict__ x, const bf16_t* __
 #pragma unroll
             for (int e = 0; e < CPL; ++e) v[e] = acc[e >> 2][i][e & 3] + tv[e];
             if (r1) {
+                const Vec16<T> r = as_loaded(rv[i]);
 #pragma unroll
-                for (int e = 0; e < CPL; ++e) v[e] += to_f(rv[i].v[e]);
+                for (int e = 0; e < CPL; ++e) v[e] += to_f(r.v[e]);
             }
             if (r2) {
+                const Vec16<T> r = as_loaded(rw[i]);
 #pragma unroll
-                for (int e = 0; e < CPL; ++e) v[e] += to_f(rw[i].v[e]);
+                for (int e = 0; e < CPL; ++e) v[e] += to_f(r.v[e]);
             }
             Vec16<T> ov;
 #pragma unroll

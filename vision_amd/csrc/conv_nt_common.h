@@ -255,8 +255,9 @@ __device__ __forceinline__ void epilogue_rows_at(f32x4_t (&acc)[NT][4], float* s
 #pragma unroll
             for (int p = 0; p < NP; ++p)
                 if (valid[i] && piece_ok[p]) {
+                    const Vec16<T> rw = as_loaded(rv[i][p]);
 #pragma unroll
-                    for (int e = 0; e < CH; ++e) acc[J0 + ((p * CH + e) >> 2)][i][e & 3] += to_f(rv[i][p].v[e]);
+                    for (int e = 0; e < CH; ++e) acc[J0 + ((p * CH + e) >> 2)][i][e & 3] += to_f(rw.v[e]);
                 }
     }
     if (r2) {
@@ -270,8 +271,9 @@ __device__ __forceinline__ void epilogue_rows_at(f32x4_t (&acc)[NT][4], float* s
 #pragma unroll
             for (int p = 0; p < NP; ++p)
                 if (valid[i] && piece_ok[p]) {
+                    const Vec16<T> rw = as_loaded(rv[i][p]);
 #pragma unroll
-                    for (int e = 0; e < CH; ++e) acc[J0 + ((p * CH + e) >> 2)][i][e & 3] += to_f(rv[i][p].v[e]);
+                    for (int e = 0; e < CH; ++e) acc[J0 + ((p * CH + e) >> 2)][i][e & 3] += to_f(rw.v[e]);
                 }
     }
     if constexpr (ACT) {                                  // piece by piece, so that only one piece's coefficients are live

@@ -173,12 +173,14 @@ thin_in_mfma_kernel(ConvGeom g, const bf16_t* __restrict__ x, const bf16_t* __re
                     for (int e = 0; e < 8; ++e) v[e] = acc[ch * 2 + (e >> 2)][e & 3];
                     const int cc = c0 + ch * 8;
                     if (res) {
+                        const Vec16<bf16_t> r = as_loaded(rv[ch]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += to_f(rv[ch].v[e]);
+                        for (int e = 0; e < 8; ++e) v[e] += to_f(r.v[e]);
                     }
                     if (res2) {
+                        const Vec16<bf16_t> r = as_loaded(rv2[ch]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += to_f(rv2[ch].v[e]);
+                        for (int e = 0; e < 8; ++e) v[e] += to_f(r.v[e]);
                     }
                     Vec16<bf16_t> ov;
 #pragma unroll
