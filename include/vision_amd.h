@@ -499,6 +499,57 @@ int vamd_image_resize_u8(const uint8_t* src, int H, int W, int pixel_bytes, cons
                          const int32_t* vbounds, const int32_t* vcoef, int vk, uint8_t* tmp, int Ho, int Wo,
                          float* dst_chw, uint8_t* dst_u8, void* stream);
 
+/* ---- serving a sequence model over codes: rotary positions, a cache in 8 bits, attention over it ------------ */
+/* No counterpart in the reference (its attention blocks see a whole image and no positions); beside vamd_timeembed and
+ * vamd_attention_fwd for models over the codebook indices of vamd_vq_forward.
+ *
+ * vamd_rotary turns pairs of the first `turned` features (even) of every head of up to two tensors x[batch][tokens][heads][dim]
+ * by positions[batch][token] * frequency, pairs (i, i + turned/2) or, interleaved, (2i, 2i+1); y1 = a (x1 cos - x2 sin),
+ * y2 = a (x2 cos + x1 sin) with a = amplitude; the other features are copied.  inverse != 0: sin -> -sin, the gradient.
+ * positions: int32, or int64 when wide != 0.  frequencies[turned/2]: turns per position as fractions of 2^64.
+ * Strides (of a batch, a token, a head) are in elements, features are adjacent; y may be x itself with the same strides, and
+ * must not overlap it otherwise.  q_heads or k_heads may be 0. */
+int vamd_rotary(const void* positions, int wide, const uint64_t* frequencies, float amplitude, int64_t batch, int64_t tokens,
+                int dim, int turned, int interleaved, int inverse, const void* q, void* yq, int q_heads, int64_t q_batch,
+                int64_t q_token, int64_t q_head, int64_t yq_batch, int64_t yq_token, int64_t yq_head, const void* k, void* yk,
+                int k_heads, int64_t k_batch, int64_t k_token, int64_t k_head, int64_t yk_batch, int64_t yk_token,
+                int64_t yk_head, int dtype, void* stream);
+
+/* The cache: codes_k, codes_v: [blocks][heads][block * dim] bytes, zero-filled once by the caller (block: 64, 128 or 256
+ * tokens; dim a multiple of 16 up to 256; the order of a block's bytes is this library's own); scales_k, scales_v:
+ * [blocks][heads] fp32, zero-filled once.  A code stands for code * scale (always a float32), scale the smallest power of two (2^-110 at least) under
+ * which the block's largest magnitude needs no code above 448 (e4m3) or 127 (int8).  table[sequence][0 .. width-1] names the
+ * blocks of a sequence (rows table_stride apart); an entry outside 0 .. blocks-1 is a hole.
+ * Batches are packed: sequence b owns rows offsets[b] .. offsets[b+1]-1, at most `most` of them, or with offsets == NULL
+ * `most` rows each (rows == sequences * most then).  Rows of no sequence are neither read nor written. */
+enum { VAMD_KV_E4M3 = 0, VAMD_KV_INT8 = 1 };
+/* Writes rows k, v [rows][heads][dim] at positions start[b], start[b]+1, ... of each sequence.  A block whose first token is
+ * written starts anew; otherwise its scale never shrinks, and its codes are moved (rounded once more) when it grows.  A block
+ * that is given an infinity or a NaN reads as NaN until it starts anew.  Rows that fall into a hole, behind `width` blocks or before
+ * position 0 (start < 0) are dropped.  A block being written belongs to one sequence of the call. */
+int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                   void* codes_k, void* codes_v, float* scales_k, float* scales_v, const int32_t* table, int64_t table_stride,
+                   const int32_t* start, const int32_t* offsets, int64_t rows, int sequences, int most, int heads, int dim,
+                   int block, int width, int blocks, int format, int dtype, void* stream);
+/* Reads the values at positions start[b], start[b]+1, ... back into rows k, v [rows][heads][dim] (exact in fp32 and in bf16);
+ * zeros for holes.  A sequence with start < 0 is left out. */
+int vamd_kv_read(const void* codes_k, const void* codes_v, const float* scales_k, const float* scales_v, const int32_t* table,
+                 int64_t table_stride, const int32_t* start, const int32_t* offsets, int64_t rows, int sequences, int most,
+                 int heads, int dim, int block, int width, int blocks, int format, void* k, int64_t k_token, int64_t k_head,
+                 void* v, int64_t v_token, int64_t v_head, int dtype, void* stream);
+/* o = softmax(scale * q k^T) v over the first lengths[b] tokens of each sequence; q, o: [rows][heads * group][dim], query head h
+ * reads key head h / group.  A sequence's queries are its last tokens: query i of n has position lengths[b] - n + i.  causal: it sees
+ * keys up to its position, with window > 0 only the last `window` of them and the first `sinks`; else all.  Tokens in
+ * holes are not seen; a query that sees nothing gives zeros.  `longest` (a bound of the lengths) only steers how the work is
+ * cut.  workspace: vamd_kv_attend_workspace bytes (may be 0), 16-byte aligned. */
+size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim);
+int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, const void* codes_k, const void* codes_v,
+                   const float* scales_k, const float* scales_v, const int32_t* table, int64_t table_stride,
+                   const int32_t* lengths, const int32_t* offsets, int64_t rows, int sequences, int most, int64_t longest,
+                   int heads, int group, int dim, int block, int width, int blocks, int format, float scale, int causal,
+                   int window, int sinks, void* o, int64_t o_token, int64_t o_head, void* workspace, size_t workspace_bytes,
+                   int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

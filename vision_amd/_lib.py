@@ -16,6 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("VAMD_LIB") or os.path.join(_HERE, "lib", "libvision_amd.so")
 
 F32, BF16 = 0, 1
+KV_E4M3, KV_INT8 = 0, 1
 ALGO_AUTO, ALGO_DIRECT, ALGO_MFMA, ALGO_THIN = 0, 1, 2, 3
 
 
@@ -158,6 +159,12 @@ SIGNATURES = {
     "vamd_vq_workspace": (_z, [_l]),
     "vamd_vq_forward": (_i, [_p, _p, _l, _i, _i, _i, _i, _f, _p, _p, _p, _p, _z, _p]),
     "vamd_vq_backward": (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _i, _f, _p, _p, _p]),
+    "vamd_rotary": (_i, [_p, _i, _p, _f, _l, _l, _i, _i, _i, _i] + [_p, _p, _i, _l, _l, _l, _l, _l, _l] * 2 + [_i, _p]),
+    "vamd_kv_append": (_i, [_p, _l, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _p, _l] + [_i] * 9 + [_p]),
+    "vamd_kv_read": (_i, [_p, _p, _p, _p, _p, _l, _p, _p, _l] + [_i] * 8 + [_p, _l, _l, _p, _l, _l, _i, _p]),
+    "vamd_kv_attend_workspace": (_z, [_i, _i, _l, _i, _i, _i]),
+    "vamd_kv_attend": (_i, [_p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _p, _l, _i, _i, _l] + [_i] * 7 +
+                       [_f, _i, _i, _i, _p, _l, _l, _p, _z, _i, _p]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():
@@ -187,3 +194,23 @@ def check(rc, what=""):
 def call(name, *args):
     """Call an int-returning entry point and raise VamdError on a non-zero status."""
     check(getattr(lib, name)(*args), name)
+
+
+def call_on(device, name, *args):
+    """The same on the current stream of `device` (its last argument), whichever device is current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+
+
+def self_overlapping(t):
+    """Whether two elements of t may share memory (as those of an expanded tensor do)."""
+    reach = 0
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return True
+        reach += stride * (size - 1)
+    return False

@@ -18,7 +18,7 @@ OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libvision_amd.so")
 PROBE_LIB = os.path.join(OUT_DIR, "libvamd_probe.so")
 SOURCES = ["elementwise.hip", "norm.hip", "conv_direct.hip", "conv_api.hip", "conv_mfma.hip", "conv_wgrad_halo.hip", "conv_thin.hip",
-           "conv_thin_mfma.hip", "attention.hip", "vq.hip", "image.hip"]
+           "conv_thin_mfma.hip", "attention.hip", "vq.hip", "image.hip", "rotary.hip", "kvcache.hip", "kv_attention.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed fp32 instructions stay off: the compiler forms them from ordinary float code, and some of their forms have given
 # wrong results on these cards now and then, without an error.

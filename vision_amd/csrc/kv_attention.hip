@@ -1,0 +1,494 @@
+// Attention of queries over a cache of 8-bit keys and values (layout, codes and scales: kv_layout.h), paged by a table of
+// blocks, for grouped heads, ragged batches, causal with an offset, optionally over a window of the last tokens and a few
+// first ones that stay visible:
+//
+//     s_j = scale * scale_k * (q . code_j) for visible j;   o = sum_j exp(s_j - m) scale_v code_j / sum_j exp(s_j - m)
+//
+// in one pass over the cache with the running maximum m, sum and output (fp32, exponents in base 2).
+//
+// kv_attend_rows_kernel: few queries (a decoding step).  A tile is up to 16 rows (query tokens x heads of one key head), so that
+// every code of the cache is read once for all heads that share it; bound by reading the cache.  Each of a workgroup's four
+// waves takes every fourth group of 64 tokens of its share of the keys; codes go straight from global memory into MFMA
+// operand order (16 bytes a lane, 1 KB a wave and load) and become bf16 in registers: code values are exact there.  With the keys as the
+// rows of the first product a lane holds 16 scores of ONE query, and exactly the slots that the second product wants as its
+// operand: nothing is exchanged but the row maximum over four lanes.  The next group's keys are loaded behind the first product, its
+// values behind the second.  The four waves' partial results meet in LDS; with more than one share per tile
+// (long contexts, small batches), they go to the workspace and a second kernel joins them.
+//
+// float32 queries: a float is the sum of three bf16 numbers, so three products with the exact codes (and three for the
+// probabilities) give fp32 accuracy on the same matrix path.
+#include "kv_layout.h"
+
+namespace vamd {
+
+struct KvAttendArgs {
+    const void* q;
+    void* o;
+    int64_t q_tok, q_head, o_tok, o_head;
+    const uint8_t* codes[2];
+    const float* scales[2];
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* offsets;
+    int64_t rows;
+    float* part;                 // [tile rows][splits][D] outputs, then [tile rows][splits][2] maximum and sum
+    float* part_ml;
+    float scale2;                // scale * log2(e)
+    int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, splits, q_aligned, o_aligned;
+};
+
+// Groups of 64 tokens that the rows of a tile can see: `sink_groups` from 0 on, then those from `first` on; `count` in all.
+struct KvRange {
+    int sink_groups, first, count;
+};
+__device__ __forceinline__ KvRange kv_range(const KvAttendArgs& a, int length, int p_first, int p_last) {
+    int hi = a.causal ? p_last + 1 : length;
+    hi = hi > length ? length : hi;
+    if (hi <= 0) return KvRange{0, 0, 0};
+    const int last = (hi + kKvGroup - 1) / kKvGroup;
+    int first = 0, sink = 0;
+    if (a.window > 0 && p_first >= a.window) {
+        first = (p_first - a.window + 1) / kKvGroup;
+        const int s = a.sinks < hi ? a.sinks : hi;
+        sink = (s + kKvGroup - 1) / kKvGroup;
+        if (sink > first) sink = first;
+    }
+    return KvRange{sink, first, sink + last - first};
+}
+// The share of `split`: at least 8 groups, so that short sequences of a batch do not fall into crumbs.
+__device__ __forceinline__ int kv_share(int count, int splits) {
+    const int per = (count + splits - 1) / splits;
+    return per < 8 ? 8 : per;
+}
+__device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
+    const int64_t room = (int64_t)a.width << a.block_shift;
+    int n = a.lengths[b];
+    n = n < 0 ? 0 : n;
+    return n > room ? (int)room : n;
+}
+
+__device__ __forceinline__ float kv_over_groups_max(float v) {           // over the four lanes that hold one query's keys
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float kv_over_groups_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+__device__ __forceinline__ float kv_finite(float m) { return m == -INFINITY ? 0.f : m; }
+
+// v as the sum of N bf16 numbers, the largest first
+template <int N> __device__ __forceinline__ void kv_pieces(float v, bf16_t (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        p[i] = (bf16_t)v;
+        v -= (float)p[i];
+    }
+}
+
+// C: 64-feature chunks of a head (the last one may be partly empty).
+template <typename T, int FMT, int C>
+__global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs a) {
+    constexpr int N = sizeof(T) == 4 ? 3 : 1;                            // bf16 pieces of a query or probability
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    int64_t id = blockIdx.x;
+    const int split = (int)(id % a.splits);
+    id /= a.splits;
+    const int64_t slot = id * 16;
+    const int tile = (int)(id % a.tiles);
+    id /= a.tiles;
+    const int h = (int)(id % a.heads), b = (int)(id / a.heads);
+
+    const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
+    if (tile * 16 >= rows.count * a.group) return;
+    const int length = kv_length(a, b);
+    const int shift = length - rows.count;                               // position of the sequence's first query
+    const int row = tile * 16 + r, tok = row / a.group;
+    const bool live = tok < rows.count;
+    const int pos = a.causal ? shift + tok : length - 1;
+    int last_row = tile * 16 + 15;
+    last_row = last_row < rows.count * a.group ? last_row : rows.count * a.group - 1;
+    const int p_first = a.causal ? shift + tile * 16 / a.group : length - 1, p_last = a.causal ? shift + last_row / a.group : length - 1;
+    const KvRange range = kv_range(a, length, p_first, p_last);
+    const int per = kv_share(range.count, a.splits);
+    const int begin = split * per, end = begin + per < range.count ? begin + per : range.count;
+    if (split > 0 && begin >= range.count) return;
+
+    const int head = h * a.group + row % a.group;
+    const int S = a.D >> 4;
+    kv_bf16x8 qf[N][C * 2];
+    {
+        const T* q = (const T*)a.q + (rows.first + (live ? tok : 0)) * a.q_tok + head * a.q_head;
+#pragma unroll
+        for (int c = 0; c < C * 2; ++c) {
+            const int d = (c >> 1) * 64 + g * 16 + (c & 1) * 8;
+            float v[8] = {};
+            if (live && d < a.D) {
+                if (a.q_aligned) {
+#pragma unroll
+                    for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
+                        const Vec16<T> w = *(const Vec16<T>*)(q + d + i * Vec16<T>::N);
+#pragma unroll
+                        for (int e = 0; e < Vec16<T>::N; ++e) v[i * Vec16<T>::N + e] = to_f(w.v[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = to_f(q[d + e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16_t p[N];
+                kv_pieces<N>(v[e], p);
+#pragma unroll
+                for (int n = 0; n < N; ++n) qf[n][c][e] = p[n];
+            }
+        }
+    }
+
+    kv_f32x4 acc[C * 4];
+#pragma unroll
+    for (int t = 0; t < C * 4; ++t) acc[t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    // page, bytes and scales of the group with running number x; a hole in the table has page -1
+    auto group_of = [&](int x) { return x < range.sink_groups ? x : x - range.sink_groups + range.first; };
+    auto page_of = [&](int x) {
+        return x < end ? kv_page(a.table, a.table_stride, a.width, a.blocks, b, group_of(x) >> (a.block_shift - 6)) : -1;
+    };
+    auto bytes_of = [&](int kv, int page, int x) {
+        const int in_block = group_of(x) & ((1 << (a.block_shift - 6)) - 1);
+        return a.codes[kv] + ((((int64_t)page * a.heads + h) << a.block_shift) + in_block * kKvGroup) * a.D;
+    };
+    kv_u32x4 kc[4 * C], vc[4 * C];
+    float ks = 0.f, vs = 0.f;
+    // in a last chunk that the head does not fill, lanes without a slab read the chunk's first one: their queries are zero
+    const int k_lane = lane * 16, k_lane_last = ((C - 1) * 4 + g < S ? lane : r) * 16;
+    auto load_k = [&](int page, int x) {
+        if (page < 0) return;
+        const uint8_t* p = bytes_of(0, page, x);
+        ks = a.scales[0][(int64_t)page * a.heads + h];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < C; ++c) kc[t * C + c] = *(const kv_u32x4*)(p + (t * S + c * 4) * 256 + (c < C - 1 ? k_lane : k_lane_last));
+    };
+    auto load_v = [&](int page, int x) {
+        if (page < 0) return;
+        const uint8_t* p = bytes_of(1, page, x) + lane * 16;
+        vs = a.scales[1][(int64_t)page * a.heads + h];
+#pragma unroll
+        for (int s = 0; s < 4 * C; ++s)
+            if (s < S) vc[s] = *(const kv_u32x4*)(p + s * 1024);
+    };
+    int x = begin + wave;
+    int page = page_of(x), next = page_of(x + 4);
+    load_k(page, x);
+    load_v(page, x);
+    for (; x < end; x += 4) {
+        const int after = page_of(x + 8);
+        if (page < 0) {
+            page = next;
+            next = after;
+            load_k(page, x + 4);
+            load_v(page, x + 4);
+            continue;
+        }
+        kv_f32x4 sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            sc[t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C * 2; ++c) {
+                const kv_u32x4 w = kc[t * C + (c >> 1)];
+                const kv_bf16x8 kf = kv_operand8<FMT>(w[(c & 1) * 2], w[(c & 1) * 2 + 1]);
+#pragma unroll
+                for (int n = N - 1; n >= 0; --n) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][c], sc[t], 0, 0, 0);
+            }
+        }
+        const float f = a.scale2 * ks, v_scale = vs;
+        const int k0 = group_of(x) * kKvGroup;
+        load_k(next, x + 4);
+        // keys that some row of the tile does not see?
+        const bool edge = k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
+                          (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float s = sc[t][i] * f;
+                if (edge) {
+                    const int j = k0 + t * 16 + g * 4 + i;
+                    const bool seen = j <= pos && j < length && (a.window <= 0 || j < a.sinks || pos - j < a.window);
+                    s = seen ? s : -INFINITY;
+                }
+                sc[t][i] = s;
+                top = fmaxf(top, s);
+            }
+        top = kv_over_groups_max(top);
+        const float m_new = fmaxf(m, top), m_use = kv_finite(m_new);
+        if (__any(m_new != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < C * 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] *= alpha;
+        }
+        m = m_new;
+        kv_bf16x8 pf[N][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(sc[t][i] - m_use);
+                l += e;
+                // the value block's scale goes into the probability: a power of two, nothing is rounded by it.  A block that reads
+                // as NaN is NaN only to the rows that see it
+                const float w = e == 0.f ? 0.f : e * v_scale;
+                bf16_t p[N];
+                kv_pieces<N>(w, p);
+#pragma unroll
+                for (int n = 0; n < N; ++n) pf[n][t >> 1][(t & 1) * 4 + i] = p[n];
+            }
+#pragma unroll
+        for (int s = 0; s < C * 4; ++s) {
+            if (s < S) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const kv_bf16x8 vf = kv_operand8<FMT>(vc[s][u * 2], vc[s][u * 2 + 1]);
+#pragma unroll
+                    for (int n = N - 1; n >= 0; --n) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u], acc[s], 0, 0, 0);
+                }
+            }
+        }
+        load_v(next, x + 4);
+        page = next;
+        next = after;
+    }
+    l = kv_over_groups_sum(l);
+
+    // the four waves' results: 2 and 3 hand theirs to 0 and 1, then 1 to 0
+    float* box_ml = lds + 2 * 64 * C * 16;
+#pragma unroll
+    for (int step = 2; step > 0; step >>= 1) {
+        if (wave >= step && wave < 2 * step) {
+            float* box = lds + (wave - step) * 64 * C * 16;
+#pragma unroll
+            for (int t = 0; t < C * 4; ++t) *(kv_f32x4*)(box + (t * 64 + lane) * 4) = acc[t];
+            box_ml[((wave - step) * 64 + lane) * 2] = m;
+            box_ml[((wave - step) * 64 + lane) * 2 + 1] = l;
+        }
+        __syncthreads();
+        if (wave < step) {
+            const float* box = lds + wave * 64 * C * 16;
+            const float m2 = box_ml[(wave * 64 + lane) * 2], l2 = box_ml[(wave * 64 + lane) * 2 + 1];
+            const float m_new = fmaxf(m, m2), m_use = kv_finite(m_new);
+            const float f1 = __builtin_amdgcn_exp2f(m - m_use), f2 = __builtin_amdgcn_exp2f(m2 - m_use);
+            m = m_new;
+            l = l * f1 + l2 * f2;
+#pragma unroll
+            for (int t = 0; t < C * 4; ++t) {
+                const kv_f32x4 o = *(const kv_f32x4*)(box + (t * 64 + lane) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] = acc[t][i] * f1 + o[i] * f2;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave > 0 || !live) return;
+    if (a.splits > 1) {
+        float* part = a.part + ((slot + r) * a.splits + split) * a.D;
+#pragma unroll
+        for (int t = 0; t < C * 4; ++t)
+            if (t < S) *(kv_f32x4*)(part + t * 16 + g * 4) = acc[t];
+        if (g == 0) {
+            float* ml = a.part_ml + ((slot + r) * a.splits + split) * 2;
+            ml[0] = m;
+            ml[1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;                          // a row that sees nothing is zero
+    T* o = (T*)a.o + (rows.first + tok) * a.o_tok + head * a.o_head;
+#pragma unroll
+    for (int t = 0; t < C * 4; ++t) {
+        if (t >= S) continue;
+        T v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = from_f<T>(acc[t][i] * inv);
+        if (a.o_aligned) {
+            if (sizeof(T) == 4) *(kv_u32x4*)(o + t * 16 + g * 4) = *(const kv_u32x4*)v;
+            else *(kv_u32x2*)(o + t * 16 + g * 4) = *(const kv_u32x2*)v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t * 16 + g * 4 + i] = v[i];
+        }
+    }
+}
+
+// Joins the shares of a row: one workgroup of 256 per row; each wave walks over every fourth share, a lane over the features.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
+    __shared__ float box[4][256], box_l[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t id = blockIdx.x;
+    const int64_t slot = id;
+    const int per_tile = a.tiles * 16;
+    const int row = (int)(id % per_tile);
+    id /= per_tile;
+    const int h = (int)(id % a.heads), b = (int)(id / a.heads);
+    const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
+    const int tok = row / a.group;
+    if (tok >= rows.count) return;
+    const int length = kv_length(a, b), shift = length - rows.count, r0 = row & ~15;
+    const int r1 = r0 + 15 < rows.count * a.group ? r0 + 15 : rows.count * a.group - 1;
+    const KvRange range = kv_range(a, length, a.causal ? shift + r0 / a.group : length - 1, a.causal ? shift + r1 / a.group : length - 1);
+    const int per = kv_share(range.count, a.splits);
+    int used = (range.count + per - 1) / per;
+    used = used < 1 ? 1 : used;
+    const float* ml = a.part_ml + slot * a.splits * 2;
+    const float* part = a.part + slot * a.splits * a.D;
+    float m = -INFINITY;
+    for (int s = lane; s < used; s += 64) m = fmaxf(m, ml[2 * s]);
+    m = kv_finite(wave_max(m));
+    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = wave; s < used; s += 4) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
+        l += ml[2 * s + 1] * f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i * 64 + lane < a.D) acc[i] += part[(int64_t)s * a.D + i * 64 + lane] * f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) box[wave][i * 64 + lane] = acc[i];
+    if (lane == 0) box_l[wave] = l;
+    __syncthreads();
+    l = (box_l[0] + box_l[1]) + (box_l[2] + box_l[3]);
+    const int d = threadIdx.x;
+    if (d >= a.D) return;
+    const float v = (box[0][d] + box[1][d]) + (box[2][d] + box[3][d]);
+    T* o = (T*)a.o + (rows.first + tok) * a.o_tok + (h * a.group + row % a.group) * a.o_head;
+    o[d] = from_f<T>(l == 0.f ? 0.f : v / l);
+}
+
+// How a call is cut: tiles of 16 rows of a (sequence, key head), and shares of the keys so that about 1024 workgroups (four a CU)
+// have work, none of them less than 8 groups of 64 tokens.
+struct KvPlan {
+    int tiles, splits;
+    int64_t slots;
+};
+static KvPlan kv_plan(int sequences, int most, int64_t longest, int heads, int group) {
+    KvPlan p;
+    p.tiles = (int)(((int64_t)most * group + 15) / 16);
+    const int64_t base = (int64_t)sequences * heads * p.tiles;
+    p.slots = base * 16;
+    const int64_t groups = (longest + kKvGroup - 1) / kKvGroup;
+    int64_t splits = base > 0 ? (1024 + base - 1) / base : 1;
+    if (splits > (groups + 7) / 8) splits = (groups + 7) / 8;
+    p.splits = splits < 1 ? 1 : splits > 256 ? 256 : (int)splits;
+    return p;
+}
+
+template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
+    const int C = (a.D + 63) / 64;
+    const size_t lds = (size_t)(2 * 64 * C * 16 + 2 * 64 * 2) * 4;
+    if (C == 1) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 1>), dim3((unsigned)grid), dim3(256), lds, st, a);
+    else if (C == 2) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 2>), dim3((unsigned)grid), dim3(256), lds, st, a);
+    else if (C == 3) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 3>), dim3((unsigned)grid), dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 4>), dim3((unsigned)grid), dim3(256), lds, st, a);
+    VAMD_LAUNCH_OK("kv_attend_rows");
+    return 0;
+}
+
+}  // namespace vamd
+
+using namespace vamd;
+
+extern "C" size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim) {
+    if (sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
+    const KvPlan p = kv_plan(sequences, most, longest, heads, group);
+    return p.splits > 1 ? (size_t)p.slots * p.splits * (dim + 2) * sizeof(float) : 0;
+}
+
+extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, const void* codes_k, const void* codes_v,
+                              const float* scales_k, const float* scales_v, const int32_t* table, int64_t table_stride,
+                              const int32_t* lengths, const int32_t* offsets, int64_t rows, int sequences, int most, int64_t longest,
+                              int heads, int group, int dim, int block, int width, int blocks, int format, float scale, int causal,
+                              int window, int sinks, void* o, int64_t o_token, int64_t o_head, void* workspace, size_t workspace_bytes,
+                              int dtype, void* stream) {
+    VAMD_REQUIRE(sequences > 0 && rows >= 0 && most >= 0 && heads > 0 && heads <= 65536 && group > 0 && group <= 65536 && width > 0 &&
+                 blocks > 0 && table_stride >= 0, "vamd_kv_attend: bad extents (%d sequences, %lld rows, most %d, %d key heads x %d, %d "
+                 "blocks a sequence of %d)", sequences, (long long)rows, most, heads, group, width, blocks);
+    VAMD_REQUIRE(dim >= 16 && dim <= 256 && dim % 16 == 0, "vamd_kv_attend: dim %d (a multiple of 16, 16 to 256)", dim);
+    VAMD_REQUIRE(block == 64 || block == 128 || block == 256, "vamd_kv_attend: block %d (64, 128 or 256 tokens)", block);
+    VAMD_REQUIRE(format == VAMD_KV_E4M3 || format == VAMD_KV_INT8, "vamd_kv_attend: bad format %d", format);
+    VAMD_REQUIRE(dtype == VAMD_F32 || dtype == VAMD_BF16, "vamd_kv_attend: bad dtype %d", dtype);
+    VAMD_REQUIRE(window >= 0 && sinks >= 0 && (causal || window == 0), "vamd_kv_attend: window %d, sinks %d (not negative; a window "
+                 "needs causal queries)", window, sinks);
+    VAMD_REQUIRE((int64_t)width * block <= 0x7fffffc0, "vamd_kv_attend: %d blocks of %d tokens are too many for a sequence", width, block);
+    VAMD_REQUIRE((int64_t)most * group <= 0x7fffffc0, "vamd_kv_attend: %d rows of %d heads are too many for a sequence", most, group);
+    VAMD_REQUIRE(offsets || rows == (int64_t)sequences * most, "vamd_kv_attend: %lld rows are not %d for each of %d sequences",
+                 (long long)rows, most, sequences);
+    if (rows == 0 || most == 0) return 0;
+    VAMD_REQUIRE(q && o && codes_k && codes_v && scales_k && scales_v && table && lengths, "vamd_kv_attend: NULL tensor");
+    const int size = dtype == VAMD_BF16 ? 2 : 4;
+    VAMD_REQUIRE((uintptr_t)codes_k % 16 == 0 && (uintptr_t)codes_v % 16 == 0 && (uintptr_t)scales_k % 4 == 0 && (uintptr_t)scales_v % 4 == 0 &&
+                 (uintptr_t)table % 4 == 0 && (uintptr_t)lengths % 4 == 0 && (uintptr_t)offsets % 4 == 0 && (uintptr_t)q % size == 0 &&
+                 (uintptr_t)o % size == 0, "vamd_kv_attend: misaligned tensor");
+    const KvPlan plan = kv_plan(sequences, most, longest, heads, group);
+    const size_t need = vamd_kv_attend_workspace(sequences, most, longest, heads, group, dim);
+    VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
+                 "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
+    const int64_t grid = plan.slots / 16 * plan.splits;
+    VAMD_REQUIRE(grid <= 0x7fffffff && plan.slots <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
+                 sequences, most);
+    KvAttendArgs a = {};
+    a.q = q;
+    a.o = o;
+    a.q_tok = q_token;
+    a.q_head = q_head;
+    a.o_tok = o_token;
+    a.o_head = o_head;
+    a.codes[0] = (const uint8_t*)codes_k;
+    a.codes[1] = (const uint8_t*)codes_v;
+    a.scales[0] = scales_k;
+    a.scales[1] = scales_v;
+    a.table = table;
+    a.table_stride = table_stride;
+    a.lengths = lengths;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.part = (float*)workspace;
+    a.part_ml = a.part + (size_t)plan.slots * plan.splits * dim;
+    a.scale2 = scale * 1.44269504088896340736f;
+    a.sequences = sequences;
+    a.most = most;
+    a.heads = heads;
+    a.group = group;
+    a.D = dim;
+    a.block_shift = block == 64 ? 6 : block == 128 ? 7 : 8;
+    a.width = width;
+    a.blocks = blocks;
+    a.window = window;
+    a.sinks = sinks;
+    a.causal = causal;
+    a.tiles = plan.tiles;
+    a.splits = plan.splits;
+    const int n = 16 / size;
+    a.q_aligned = (uintptr_t)q % 16 == 0 && q_token % n == 0 && q_head % n == 0;
+    a.o_aligned = (uintptr_t)o % (4 * size) == 0 && o_token % 4 == 0 && o_head % 4 == 0;
+    hipStream_t st = as_stream(stream);
+    int rc;
+    if (dtype == VAMD_BF16) rc = format == VAMD_KV_E4M3 ? kv_launch_rows<bf16_t, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<bf16_t, VAMD_KV_INT8>(a, grid, st);
+    else rc = format == VAMD_KV_E4M3 ? kv_launch_rows<float, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<float, VAMD_KV_INT8>(a, grid, st);
+    if (rc || plan.splits == 1) return rc;
+    if (dtype == VAMD_BF16) hipLaunchKernelGGL(kv_join_kernel<bf16_t>, dim3((unsigned)plan.slots), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(kv_join_kernel<float>, dim3((unsigned)plan.slots), dim3(256), 0, st, a);
+    VAMD_LAUNCH_OK("kv_join");
+    return 0;
+}

@@ -1,0 +1,212 @@
+"""Rotary positions for the queries and keys of attention: beside the time embedding of the UNets (`vamd_timeembed`), what a
+sequence model over codebook indices has in place of it.
+
+    rotary = Rotary(head_dim, rotary_dim, layout="half", base=10000.0, scaling={"type": "yarn", "factor": 4.0, "original": 8192})
+    q, k = rotary(positions, q, k)                 # differentiable; one kernel for both, one for both gradients
+    rotary.apply_(positions, q, k)                 # in place, without gradients
+
+q, k: [..., heads, head_dim], float32 or bfloat16 on the GPU, any strides with adjacent features (heads may come before tokens
+in memory); positions: int32 or int64, of shape q.shape[:-2] or broadcast to it.  Angles are exact fractions of a turn at any
+position (csrc/rotary.hip).  There is no CPU path.
+"""
+import math
+from fractions import Fraction
+
+import torch
+from torch import nn
+
+from . import _lib
+from ._lib import call_on, self_overlapping
+
+_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_PI = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None):
+    """(radians per position of each pair as Python floats, amplitude).
+
+    f_i = base^(-2i / rotary_dim).  Contexts longer than the trained one:
+      {"type": "linear", "factor": s}                    f / s: positions are squeezed
+      {"type": "ntk", "factor": s}                       base * s^(R / (R - 2)): the slowest pair is slowed by s, the fastest not
+      {"type": "yarn", "factor": s, "original": L}       pairs that turn less than `alpha` (1) times over L positions are slowed by
+                                                         s, those that turn more than `beta` (32) times are left alone, a linear
+                                                         blend between; the turned features grow by `amplitude` (0.1 ln s + 1)
+    """
+    R, amplitude = rotary_dim, 1.0
+    base = float(base)
+    scaling = dict(scaling) if scaling else {"type": "none"}
+    kind = scaling.pop("type", None)
+    known = {"none": (), "linear": ("factor",), "ntk": ("factor",), "yarn": ("factor", "original", "alpha", "beta", "amplitude")}
+    if kind not in known:
+        raise ValueError(f"scaling type {kind!r} (linear, ntk or yarn)")
+    odd = set(scaling) - set(known[kind])
+    if odd:
+        raise ValueError(f"scaling {kind!r} has no {sorted(odd)}")
+    factor = float(scaling["factor"]) if kind != "none" else 1.0
+    if not factor >= 1.0 or math.isinf(factor):
+        raise ValueError(f"a scaling's factor is 1 or more, not {factor}")
+    if not 1.0 < base < math.inf:
+        raise ValueError(f"base {base}: a number above 1")
+    if kind == "ntk" and R > 2:
+        base *= factor ** (R / (R - 2))
+    f = [base ** (-i / R) for i in range(0, R, 2)]
+    if kind == "linear":
+        f = [x / factor for x in f]
+    if kind == "yarn":
+        alpha, beta = float(scaling.get("alpha", 1.0)), float(scaling.get("beta", 32.0))
+        if not alpha < beta:
+            raise ValueError(f"yarn needs alpha < beta, not {alpha} and {beta}")
+        turns = [float(scaling["original"]) * x / (2 * math.pi) for x in f]
+        keep = [min(1.0, max(0.0, (r - alpha) / (beta - alpha))) for r in turns]
+        f = [x * g + x / factor * (1 - g) for x, g in zip(f, keep)]
+        amplitude = float(scaling.get("amplitude", 0.1 * math.log(factor) + 1))
+    return f, amplitude
+
+
+def _rows(t, lead=None):
+    """t as [batch, tokens, heads, dim] without a copy, with the given batch and tokens or as its strides allow; or None."""
+    n = t.dim() - 2
+    if n < 2:
+        return t[(None,) * (2 - n)]
+    if n == 2:
+        return t
+    heads = t.shape[-2:]
+    for split in ((lead,) if lead else ((t.shape[0], t.shape[1:-2].numel()), (t.shape[:-3].numel(), t.shape[-3]))):
+        try:
+            return t.view(*split, *heads)
+        except RuntimeError:
+            pass
+    return None
+
+
+def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, tensors, outs):
+    """One launch for up to two tensors of equal leading dimensions; None entries are left out."""
+    args, ref, lead = [], next(t for t in tensors if t is not None), None
+    for t, o in zip(tensors, outs):
+        if t is None:
+            args += [None, None, 0, 0, 0, 0, 0, 0, 0]
+            continue
+        a = _rows(t, lead)
+        if a is None:                                # it cannot be walked over as the first one is
+            if o is t:
+                raise ValueError(f"q and k with strides {ref.stride()} and {t.stride()} cannot be turned in place together")
+            a = _rows(t.contiguous(), lead)
+        lead = a.shape[:2]
+        b = a if o is t else _rows(o, lead)
+        s, r = a.stride(), b.stride()
+        args += [a.data_ptr(), b.data_ptr(), a.shape[2], s[0], s[1], s[2], r[0], r[1], r[2]]
+    if positions.shape != ref.shape[:-2]:
+        positions = positions.expand(ref.shape[:-2])
+    positions = positions.contiguous()
+    call_on(ref.device, "vamd_rotary", positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(), amplitude,
+            lead[0], lead[1], ref.shape[-1], turned, interleaved, inverse, *args, _TYPES[ref.dtype])
+
+
+def _readable(t):
+    return t if t is None or (t.stride(-1) == 1 and _rows(t) is not None) else t.contiguous()
+
+
+def _fresh(x):
+    """Memory for a result: x's own layout where it is dense and has few leading dimensions, else contiguous."""
+    y = torch.empty_like(x) if x.dim() <= 4 else None
+    return y if y is not None and y.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, frequencies, amplitude, turned, interleaved, inverse, q, k):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (amplitude, turned, interleaved, inverse)
+        ctx.set_materialize_grads(False)
+        xs = [_readable(q), _readable(k)]
+        outs = [None if x is None else _fresh(x) for x in xs]
+        _turn(positions, frequencies, amplitude, turned, interleaved, inverse, xs, outs)
+        return tuple(outs)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, frequencies = ctx.saved_tensors
+        amplitude, turned, interleaved, inverse = ctx.how
+        if not ctx.needs_input_grad[6]:
+            gq = None
+        if not ctx.needs_input_grad[7]:
+            gk = None
+        if gq is None and gk is None:
+            return (None,) * 8
+        # the transpose of a turn is the turn back, with the same amplitude: the same function, differentiable in turn
+        return (None,) * 6 + _RotaryFn.apply(positions, frequencies, amplitude, turned, interleaved, 1 - inverse, gq, gk)
+
+
+class Rotary(nn.Module):
+    def __init__(self, head_dim, rotary_dim=None, layout="half", base=10000.0, scaling=None, device=None):
+        super().__init__()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout {layout!r} (half or interleaved)")
+        if rotary_dim % 2 or not 2 <= rotary_dim <= head_dim:
+            raise ValueError(f"{rotary_dim} of {head_dim} features cannot be turned (an even number, 2 to the head's size)")
+        self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
+        f, self.amplitude = rotary_frequencies(rotary_dim, base, scaling)
+        # radians -> 64-bit fractions of a turn, rounded once; whole turns per position would drop out (none has any)
+        turns = [round(Fraction(x) / (2 * _PI) * 2 ** 64) % 2 ** 64 for x in f]
+        bits = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self.register_buffer("frequencies", bits, persistent=False)
+
+    def _check(self, positions, q, k):
+        for name, t in (("q", q), ("k", k)):
+            if t is None:
+                continue
+            if t.dtype not in _TYPES:
+                raise TypeError(f"{name} is {t.dtype}: float32 or bfloat16")
+            if t.dim() < 2 or t.shape[-1] != self.head_dim:
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, not [..., heads, {self.head_dim}]")
+        if k is not None and (k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2] or k.device != q.device):
+            raise ValueError(f"q and k differ: {q.dtype} {tuple(q.shape)} on {q.device}, {k.dtype} {tuple(k.shape)} on {k.device}")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions are {positions.dtype}: int32 or int64")
+        lead, have = q.shape[:-2], positions.shape
+        if have != lead and (len(have) > len(lead) or any(n not in (1, m) for n, m in zip(reversed(have), reversed(lead)))):
+            raise ValueError(f"positions have shape {tuple(have)}, not {tuple(lead)} or broadcast to it")
+        if not q.is_cuda:
+            raise RuntimeError("Rotary runs on the GPU only (libvision_amd.so has no CPU path)")
+        if positions.device != q.device or self.frequencies.device != q.device:
+            raise ValueError(f"q is on {q.device}, positions on {positions.device}, the frequencies on {self.frequencies.device}")
+
+    def forward(self, positions, q, k=None):
+        self._check(positions, q, k)
+        if q.numel() == 0 or (k is not None and k.numel() == 0):
+            if k is None:
+                return q.clone()
+            if q.numel() == 0 and k.numel() == 0:
+                return q.clone(), k.clone()
+            return (self(positions, q), k.clone()) if k.numel() == 0 else (q.clone(), self(positions, k))
+        how = (self.amplitude, self.rotary_dim, int(self.layout == "interleaved"), 0)
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            yq, yk = _RotaryFn.apply(positions, self.frequencies, *how, q, k)
+        else:
+            xs = (_readable(q), _readable(k))
+            yq, yk = (None if x is None else _fresh(x) for x in xs)
+            _turn(positions, self.frequencies, *how, xs, (yq, yk))
+        return yq if k is None else (yq, yk)
+
+    def apply_(self, positions, q, k=None):
+        """Turns q and k in place and returns them; for inference (no gradient passes through it)."""
+        self._check(positions, q, k)
+        for name, t in (("q", q), ("k", k)):
+            if t is None:
+                continue
+            if torch.is_grad_enabled() and t.requires_grad:
+                raise RuntimeError(f"{name} requires a gradient: apply_ is not differentiable, call the module instead")
+            if t.numel() and (t.stride(-1) != 1 or _rows(t) is None or self_overlapping(t)):
+                raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
+        if k is not None and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("q and k are the same memory")
+        for t in (q, k):
+            if t is not None and t.numel() and not t.is_inference():
+                torch.autograd.graph.increment_version(t)
+        if q.numel() == 0 or (k is not None and k.numel() == 0):
+            if k is not None and (q.numel() or k.numel()):
+                self.apply_(positions, q if q.numel() else k)
+            return q if k is None else (q, k)
+        _turn(positions, self.frequencies, self.amplitude, self.rotary_dim, int(self.layout == "interleaved"), 0, (q, k), (q, k))
+        return q if k is None else (q, k)
