@@ -196,14 +196,19 @@ def call(name, *args):
     check(getattr(lib, name)(*args), name)
 
 
+_entries = {name: getattr(lib, name) for name in SIGNATURES}
+
+
 def call_on(device, name, *args):
     """The same on the current stream of `device` (its last argument), whichever device is current."""
     index = device.index
     if index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+        rc = _entries[name](*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+            rc = _entries[name](*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 def self_overlapping(t):

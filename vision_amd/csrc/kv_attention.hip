@@ -56,10 +56,11 @@ __device__ __forceinline__ KvRange kv_range(const KvAttendArgs& a, int length, i
     }
     return KvRange{sink, first, sink + last - first};
 }
-// The share of `split`: at least 8 groups, so that short sequences of a batch do not fall into crumbs.
+// The share of a split: at least 8 groups, so that short sequences of a batch do not fall into crumbs.
+constexpr int kKvMinShare = 8;
 __device__ __forceinline__ int kv_share(int count, int splits) {
     const int per = (count + splits - 1) / splits;
-    return per < 8 ? 8 : per;
+    return per < kKvMinShare ? kKvMinShare : per;
 }
 __device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
     const int64_t room = (int64_t)a.width << a.block_shift;
@@ -87,20 +88,27 @@ template <int N> __device__ __forceinline__ void kv_pieces(float v, bf16_t (&p)[
     }
 }
 
+// The codes as the loads left them, opaque to the compiler until here: it would convert all of a group's codes where they
+// arrive, which takes four times their registers.
+__device__ __forceinline__ kv_u32x4 kv_as_loaded(kv_u32x4 w) {
+    asm("" : "+v"(w));
+    return w;
+}
+
 // C: 64-feature chunks of a head (the last one may be partly empty).
 template <typename T, int FMT, int C>
-__global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(const KvAttendArgs a) {
     constexpr int N = sizeof(T) == 4 ? 3 : 1;                            // bf16 pieces of a query or probability
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    int64_t id = blockIdx.x;
-    const int split = (int)(id % a.splits);
-    id /= a.splits;
-    const int64_t slot = id * 16;
-    const int tile = (int)(id % a.tiles);
-    id /= a.tiles;
-    const int h = (int)(id % a.heads), b = (int)(id / a.heads);
+    uint32_t id = blockIdx.x;
+    const int split = (int)(id % (uint32_t)a.splits);
+    id /= (uint32_t)a.splits;
+    const int64_t slot = (int64_t)id * 16;
+    const int tile = (int)(id % (uint32_t)a.tiles);
+    id /= (uint32_t)a.tiles;
+    const int h = (int)(id % (uint32_t)a.heads), b = (int)(id / (uint32_t)a.heads);
 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     if (tile * 16 >= rows.count * a.group) return;
@@ -117,34 +125,26 @@ __global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs 
     const int begin = split * per, end = begin + per < range.count ? begin + per : range.count;
     if (split > 0 && begin >= range.count) return;
 
-    const int head = h * a.group + row % a.group;
+    const int head = h * a.group + row - tok * a.group;
     const int S = a.D >> 4;
-    kv_bf16x8 qf[N][C * 2];
+    // the queries' loads are issued before the first keys' and taken apart behind them
+    Vec16<T> q_raw[C * 2][8 / Vec16<T>::N];
     {
         const T* q = (const T*)a.q + (rows.first + (live ? tok : 0)) * a.q_tok + head * a.q_head;
 #pragma unroll
         for (int c = 0; c < C * 2; ++c) {
             const int d = (c >> 1) * 64 + g * 16 + (c & 1) * 8;
-            float v[8] = {};
-            if (live && d < a.D) {
-                if (a.q_aligned) {
 #pragma unroll
-                    for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
-                        const Vec16<T> w = *(const Vec16<T>*)(q + d + i * Vec16<T>::N);
+            for (int i = 0; i < 8 / Vec16<T>::N; ++i) {
+                q_raw[c][i] = Vec16<T>{};
+                if (live && d < a.D) {
+                    const T* p = q + d + i * Vec16<T>::N;
+                    if (a.q_aligned) q_raw[c][i] = *(const Vec16<T>*)p;
+                    else {
 #pragma unroll
-                        for (int e = 0; e < Vec16<T>::N; ++e) v[i * Vec16<T>::N + e] = to_f(w.v[e]);
+                        for (int e = 0; e < Vec16<T>::N; ++e) q_raw[c][i].v[e] = p[e];
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = to_f(q[d + e]);
                 }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                bf16_t p[N];
-                kv_pieces<N>(v[e], p);
-#pragma unroll
-                for (int n = 0; n < N; ++n) qf[n][c][e] = p[n];
             }
         }
     }
@@ -154,81 +154,103 @@ __global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs 
     for (int t = 0; t < C * 4; ++t) acc[t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    // page, bytes and scales of the group with running number x; a hole in the table has page -1
+    // The group with running number x: its block (block 0 in place of a hole, none of whose tokens is seen), its bytes.
     auto group_of = [&](int x) { return x < range.sink_groups ? x : x - range.sink_groups + range.first; };
     auto page_of = [&](int x) {
         return x < end ? kv_page(a.table, a.table_stride, a.width, a.blocks, b, group_of(x) >> (a.block_shift - 6)) : -1;
     };
+    auto at_of = [&](int page) { return (int64_t)(page < 0 ? 0 : page) * a.heads + h; };
     auto bytes_of = [&](int kv, int page, int x) {
         const int in_block = group_of(x) & ((1 << (a.block_shift - 6)) - 1);
-        return a.codes[kv] + ((((int64_t)page * a.heads + h) << a.block_shift) + in_block * kKvGroup) * a.D;
+        return a.codes[kv] + ((at_of(page) << a.block_shift) + in_block * kKvGroup) * a.D;
     };
     kv_u32x4 kc[4 * C], vc[4 * C];
     float ks = 0.f, vs = 0.f;
     // in a last chunk that the head does not fill, lanes without a slab read the chunk's first one: their queries are zero
     const int k_lane = lane * 16, k_lane_last = ((C - 1) * 4 + g < S ? lane : r) * 16;
     auto load_k = [&](int page, int x) {
-        if (page < 0) return;
         const uint8_t* p = bytes_of(0, page, x);
-        ks = a.scales[0][(int64_t)page * a.heads + h];
+        ks = a.scales[0][at_of(page)];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < C; ++c) kc[t * C + c] = *(const kv_u32x4*)(p + (t * S + c * 4) * 256 + (c < C - 1 ? k_lane : k_lane_last));
     };
     auto load_v = [&](int page, int x) {
-        if (page < 0) return;
-        const uint8_t* p = bytes_of(1, page, x) + lane * 16;
-        vs = a.scales[1][(int64_t)page * a.heads + h];
+        const uint8_t* p = bytes_of(1, page, x);
+        vs = a.scales[1][at_of(page)];
 #pragma unroll
         for (int s = 0; s < 4 * C; ++s)
-            if (s < S) vc[s] = *(const kv_u32x4*)(p + s * 1024);
+            if (s < S) vc[s] = *(const kv_u32x4*)(p + s * 1024 + k_lane);
     };
     int x = begin + wave;
     int page = page_of(x), next = page_of(x + 4);
-    load_k(page, x);
-    load_v(page, x);
+    if (x < end) {
+        load_k(page, x);
+        load_v(page, x);
+    }
+    kv_bf16x8 qf[N][C * 2];
+#pragma unroll
+    for (int c = 0; c < C * 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const T v = q_raw[c][e / Vec16<T>::N].v[e % Vec16<T>::N];
+            if constexpr (N == 1) qf[0][c][e] = v;
+            else {
+                bf16_t p[N];
+                kv_pieces<N>(v, p);
+#pragma unroll
+                for (int n = 0; n < N; ++n) qf[n][c][e] = p[n];
+            }
+        }
+    // what this lane's query sees: keys up to `upto`, from `from` on or below `first_keys`
+    const int upto = pos < length ? pos : length - 1, from = a.window > 0 ? pos - a.window + 1 : 0, first_keys = a.window > 0 ? a.sinks : 0;
     for (; x < end; x += 4) {
         const int after = page_of(x + 8);
-        if (page < 0) {
-            page = next;
-            next = after;
-            load_k(page, x + 4);
-            load_v(page, x + 4);
-            continue;
-        }
+        const bool more = x + 4 < end;
         kv_f32x4 sc[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             sc[t] = kv_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < C * 2; ++c) {
-                const kv_u32x4 w = kc[t * C + (c >> 1)];
-                const kv_bf16x8 kf = kv_operand8<FMT>(w[(c & 1) * 2], w[(c & 1) * 2 + 1]);
+            for (int c = 0; c < C; ++c) {
+                const kv_u32x4 w = kv_as_loaded(kc[t * C + c]);
 #pragma unroll
-                for (int n = N - 1; n >= 0; --n) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][c], sc[t], 0, 0, 0);
+                for (int u = 0; u < 2; ++u) {
+                    const kv_bf16x8 kf = kv_operand8<FMT>(w[u * 2], w[u * 2 + 1]);
+#pragma unroll
+                    for (int n = N - 1; n >= 0; --n) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][c * 2 + u], sc[t], 0, 0, 0);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         const float f = a.scale2 * ks, v_scale = vs;
         const int k0 = group_of(x) * kKvGroup;
-        load_k(next, x + 4);
+        if (more) load_k(next, x + 4);
         // keys that some row of the tile does not see?
-        const bool edge = k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
+        const bool edge = page < 0 || k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
                           (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][i] *= f;
+        if (edge) {
+            const int k_lane0 = k0 + g * 4;
+            const int rel_upto = page < 0 ? -1 : upto - k_lane0, rel_from = from - k_lane0, rel_first = first_keys - k_lane0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = t * 16 + i;
+                    const bool seen = j <= rel_upto && (j >= rel_from || j < rel_first);
+                    sc[t][i] = seen ? sc[t][i] : -INFINITY;
+                }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float s = sc[t][i] * f;
-                if (edge) {
-                    const int j = k0 + t * 16 + g * 4 + i;
-                    const bool seen = j <= pos && j < length && (a.window <= 0 || j < a.sinks || pos - j < a.window);
-                    s = seen ? s : -INFINITY;
-                }
-                sc[t][i] = s;
-                top = fmaxf(top, s);
-            }
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
         top = kv_over_groups_max(top);
         const float m_new = fmaxf(m, top), m_use = kv_finite(m_new);
         if (__any(m_new != m)) {
@@ -240,33 +262,48 @@ __global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs 
                 for (int i = 0; i < 4; ++i) acc[t][i] *= alpha;
         }
         m = m_new;
-        kv_bf16x8 pf[N][2];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = __builtin_amdgcn_exp2f(sc[t][i] - m_use);
                 l += e;
-                // the value block's scale goes into the probability: a power of two, nothing is rounded by it.  A block that reads
-                // as NaN is NaN only to the rows that see it
-                const float w = e == 0.f ? 0.f : e * v_scale;
+                sc[t][i] = e * v_scale;          // the values' scale goes into the probability: a power of two, nothing is rounded
+            }
+        if (v_scale != v_scale) {                // a block that reads as NaN is NaN only to the queries that see it
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = k0 + t * 16 + g * 4 + i;
+                    const bool seen = page >= 0 && j <= upto && (j >= from || j < first_keys);
+                    sc[t][i] = seen ? sc[t][i] : 0.f;
+                }
+        }
+        kv_bf16x8 pf[N][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
                 bf16_t p[N];
-                kv_pieces<N>(w, p);
+                kv_pieces<N>(sc[t][i], p);
 #pragma unroll
                 for (int n = 0; n < N; ++n) pf[n][t >> 1][(t & 1) * 4 + i] = p[n];
             }
 #pragma unroll
         for (int s = 0; s < C * 4; ++s) {
             if (s < S) {
+                const kv_u32x4 w = kv_as_loaded(vc[s]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const kv_bf16x8 vf = kv_operand8<FMT>(vc[s][u * 2], vc[s][u * 2 + 1]);
+                    const kv_bf16x8 vf = kv_operand8<FMT>(w[u * 2], w[u * 2 + 1]);
 #pragma unroll
                     for (int n = N - 1; n >= 0; --n) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][u], acc[s], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        load_v(next, x + 4);
+        if (more) load_v(next, x + 4);
         page = next;
         next = after;
     }
@@ -331,17 +368,20 @@ __global__ void __launch_bounds__(256) kv_attend_rows_kernel(const KvAttendArgs 
     }
 }
 
-// Joins the shares of a row: one workgroup of 256 per row; each wave walks over every fourth share, a lane over the features.
-template <typename T>
-__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
-    __shared__ float box[4][256], box_l[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t id = blockIdx.x;
-    const int64_t slot = id;
-    const int per_tile = a.tiles * 16;
-    const int row = (int)(id % per_tile);
-    id /= per_tile;
-    const int h = (int)(id % a.heads), b = (int)(id / a.heads);
+// Joins the shares of a row: one workgroup of 16 waves per row.  The shares' weights go to LDS first, so that the loads of the
+// outputs depend on nothing; a lane then reads four features of every (1024 / lanes a row takes)-th share, eight in flight.
+constexpr int kKvMaxSplits = 256;
+template <typename T, int kKvJoin>
+__global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) {
+    __shared__ float weight[kKvMaxSplits], box_m[4], box_l[4];
+    __shared__ __attribute__((aligned(16))) float box[kKvJoin * 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t id = blockIdx.x;
+    const uint32_t per_head = (uint32_t)a.most * a.group;
+    const int row = (int)(id % per_head);
+    id /= per_head;
+    const int64_t slot = (int64_t)id * a.tiles * 16 + row;
+    const int h = (int)(id % (uint32_t)a.heads), b = (int)(id / (uint32_t)a.heads);
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int tok = row / a.group;
     if (tok >= rows.count) return;
@@ -352,32 +392,53 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttendArgs a) {
     int used = (range.count + per - 1) / per;
     used = used < 1 ? 1 : used;
     const float* ml = a.part_ml + slot * a.splits * 2;
-    const float* part = a.part + slot * a.splits * a.D;
-    float m = -INFINITY;
-    for (int s = lane; s < used; s += 64) m = fmaxf(m, ml[2 * s]);
-    m = kv_finite(wave_max(m));
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = wave; s < used; s += 4) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-        l += ml[2 * s + 1] * f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i * 64 + lane < a.D) acc[i] += part[(int64_t)s * a.D + i * 64 + lane] * f;
+    for (int i = 0; i < kKvMaxSplits / 64; ++i) {
+        if (i % (kKvJoin / 64) != wave) continue;
+        const int s = i * 64 + lane;
+        const float m0 = s < used ? ml[2 * s] : -INFINITY, l0 = s < used ? ml[2 * s + 1] : 0.f;
+        const float m1 = wave_max(m0), w = __builtin_amdgcn_exp2f(m0 - kv_finite(m1));
+        weight[s] = w;                                           // relative to the largest of its 64 shares
+        const float l1 = wave_sum(l0 * w);
+        if (lane == 0) {
+            box_m[i] = m1;
+            box_l[i] = l1;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) box[wave][i * 64 + lane] = acc[i];
-    if (lane == 0) box_l[wave] = l;
     __syncthreads();
-    l = (box_l[0] + box_l[1]) + (box_l[2] + box_l[3]);
-    const int d = threadIdx.x;
-    if (d >= a.D) return;
-    const float v = (box[0][d] + box[1][d]) + (box[2][d] + box[3][d]);
-    T* o = (T*)a.o + (rows.first + tok) * a.o_tok + (h * a.group + row % a.group) * a.o_head;
-    o[d] = from_f<T>(l == 0.f ? 0.f : v / l);
+    const float m = kv_finite(fmaxf(fmaxf(box_m[0], box_m[1]), fmaxf(box_m[2], box_m[3])));
+    float f[4], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = __builtin_amdgcn_exp2f(box_m[i] - m);
+        l += box_l[i] * f[i];
+    }
+    const int quads = a.D >> 2, lines = kKvJoin / quads;         // lanes of a row; rows (shares) read at once
+    const int line = tid / quads, d = tid % quads * 4;
+    kv_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (line < lines) {
+        const float* p = a.part + slot * a.splits * a.D + d;
+#pragma unroll 8
+        for (int s = line; s < used; s += lines) {
+            const float w = weight[s] * f[s >> 6];
+            const kv_f32x4 v = *(const kv_f32x4*)(p + (int64_t)s * a.D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += v[e] * w;
+        }
+    }
+    *(kv_f32x4*)(box + tid * 4) = acc;
+    __syncthreads();
+    T* o = (T*)a.o + (rows.first + tok) * a.o_tok + (h * a.group + row - tok * a.group) * a.o_head;
+    for (int e = tid; e < a.D; e += kKvJoin) {
+        float v = 0.f;
+        for (int i = 0; i < lines && i < used; ++i) v += box[(i * quads + (e >> 2)) * 4 + (e & 3)];
+        o[e] = from_f<T>(l == 0.f ? 0.f : v / l);
+    }
 }
 
-// How a call is cut: tiles of 16 rows of a (sequence, key head), and shares of the keys so that about 1024 workgroups (four a CU)
-// have work, none of them less than 8 groups of 64 tokens.
+// How a call is cut: tiles of 16 rows of a (sequence, key head), and shares of the keys so that 512 workgroups (two a CU, all
+// resident) have work, none of them less than 8 groups of 64 tokens.  One token of 64 sequences of up to 4096 (8 key heads, 128
+// features): 61 us with 256 or 512, 65 with 768, 79 with 1024 workgroups; of one sequence of 131071: 40, 42, 47 and 46 us.
 struct KvPlan {
     int tiles, splits;
     int64_t slots;
@@ -388,20 +449,37 @@ static KvPlan kv_plan(int sequences, int most, int64_t longest, int heads, int g
     const int64_t base = (int64_t)sequences * heads * p.tiles;
     p.slots = base * 16;
     const int64_t groups = (longest + kKvGroup - 1) / kKvGroup;
-    int64_t splits = base > 0 ? (1024 + base - 1) / base : 1;
-    if (splits > (groups + 7) / 8) splits = (groups + 7) / 8;
-    p.splits = splits < 1 ? 1 : splits > 256 ? 256 : (int)splits;
+    int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
+    if (splits > (groups + kKvMinShare - 1) / kKvMinShare) splits = (groups + kKvMinShare - 1) / kKvMinShare;
+    p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
     return p;
 }
 
 template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
     const int C = (a.D + 63) / 64;
     const size_t lds = (size_t)(2 * 64 * C * 16 + 2 * 64 * 2) * 4;
-    if (C == 1) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 1>), dim3((unsigned)grid), dim3(256), lds, st, a);
-    else if (C == 2) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 2>), dim3((unsigned)grid), dim3(256), lds, st, a);
-    else if (C == 3) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 3>), dim3((unsigned)grid), dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, 4>), dim3((unsigned)grid), dim3(256), lds, st, a);
+#define KV_ROWS(C_)                                                                                                              \
+    case C_: hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_>), dim3((unsigned)grid), dim3(256), lds, st, a); break
+    switch (C) {
+        KV_ROWS(1);
+        KV_ROWS(2);
+        KV_ROWS(3);
+        KV_ROWS(4);
+    }
+#undef KV_ROWS
     VAMD_LAUNCH_OK("kv_attend_rows");
+    return 0;
+}
+
+// One wave per row, four or sixteen: so many that a lane reads about four shares.  32 rows of 256 shares: 12 us with four waves, 5.8 with
+// sixteen; 512 rows of 4 shares (128 features): 18 us with sixteen waves, 4 with one.
+template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream_t st) {
+    const unsigned grid = (unsigned)((int64_t)a.sequences * a.heads * a.most * a.group);
+    const int lanes = a.splits * (a.D / 4) / 4;
+    if (lanes <= 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), dim3(grid), dim3(64), 0, st, a);
+    else if (lanes <= 256) hipLaunchKernelGGL((kv_join_kernel<T, 256>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv_join_kernel<T, 1024>), dim3(grid), dim3(1024), 0, st, a);
+    VAMD_LAUNCH_OK("kv_join");
     return 0;
 }
 
@@ -487,8 +565,5 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     if (dtype == VAMD_BF16) rc = format == VAMD_KV_E4M3 ? kv_launch_rows<bf16_t, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<bf16_t, VAMD_KV_INT8>(a, grid, st);
     else rc = format == VAMD_KV_E4M3 ? kv_launch_rows<float, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<float, VAMD_KV_INT8>(a, grid, st);
     if (rc || plan.splits == 1) return rc;
-    if (dtype == VAMD_BF16) hipLaunchKernelGGL(kv_join_kernel<bf16_t>, dim3((unsigned)plan.slots), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(kv_join_kernel<float>, dim3((unsigned)plan.slots), dim3(256), 0, st, a);
-    VAMD_LAUNCH_OK("kv_join");
-    return 0;
+    return dtype == VAMD_BF16 ? kv_launch_join<bf16_t>(a, st) : kv_launch_join<float>(a, st);
 }

@@ -112,12 +112,13 @@ class KVCache:
             if rows < 0:
                 raise ValueError(f"{rows} rows")
             shape = (rows, self.kv_heads, self.head_dim)
-            out = (torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device))
-        k, v = out
-        for name, t in (("out[0]", k), ("out[1]", v)):
-            self._written(name, t, (rows, self.kv_heads, self.head_dim))
-        if k.dtype != v.dtype or k.data_ptr() == v.data_ptr() and k.numel():
-            raise ValueError("out: two different tensors of one dtype")
+            k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        else:
+            k, v = out
+            for name, t in (("out[0]", k), ("out[1]", v)):
+                self._written(name, t, (rows, self.kv_heads, self.head_dim))
+            if k.dtype != v.dtype or k.data_ptr() == v.data_ptr() and k.numel():
+                raise ValueError("out: two different tensors of one dtype")
         n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
         call_on(self.device, "vamd_kv_read", *self._pointers, table.data_ptr(), table.stride(0), start.data_ptr(),

@@ -63,78 +63,96 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None):
     return f, amplitude
 
 
-def _rows(t, lead=None):
-    """t as [batch, tokens, heads, dim] without a copy, with the given batch and tokens or as its strides allow; or None."""
-    n = t.dim() - 2
-    if n < 2:
-        return t[(None,) * (2 - n)]
+def _layout(t, lead=None):
+    """(batch, tokens, batch stride, token stride, head stride) of t [..., heads, dim] as a launch walks over it, with the given
+    (batch, tokens) or as its strides allow; None if no such walk exists."""
+    s, n = t.stride(), t.dim()
+    if n == 3:
+        return 1, t.shape[0], 0, s[0], s[1]
+    if n == 4:
+        return t.shape[0], t.shape[1], s[0], s[1], s[2]
     if n == 2:
-        return t
+        return 1, 1, 0, 0, s[0]
     heads = t.shape[-2:]
     for split in ((lead,) if lead else ((t.shape[0], t.shape[1:-2].numel()), (t.shape[:-3].numel(), t.shape[-3]))):
         try:
-            return t.view(*split, *heads)
+            s = t.view(*split, *heads).stride()
+            return (*split, s[0], s[1], s[2])
         except RuntimeError:
             pass
     return None
 
 
-def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, tensors, outs):
-    """One launch for up to two tensors of equal leading dimensions; None entries are left out."""
-    args, ref, lead = [], next(t for t in tensors if t is not None), None
-    for t, o in zip(tensors, outs):
-        if t is None:
-            args += [None, None, 0, 0, 0, 0, 0, 0, 0]
-            continue
-        a = _rows(t, lead)
-        if a is None:                                # it cannot be walked over as the first one is
-            if o is t:
-                raise ValueError(f"q and k with strides {ref.stride()} and {t.stride()} cannot be turned in place together")
-            a = _rows(t.contiguous(), lead)
-        lead = a.shape[:2]
-        b = a if o is t else _rows(o, lead)
-        s, r = a.stride(), b.stride()
-        args += [a.data_ptr(), b.data_ptr(), a.shape[2], s[0], s[1], s[2], r[0], r[1], r[2]]
-    if positions.shape != ref.shape[:-2]:
+def _args(t, o, lead):
+    """What the entry point wants to know of one tensor and its result; (arguments, (batch, tokens))."""
+    a = _layout(t, lead)
+    if a is None:                                    # it cannot be walked over as the first one is
+        if o is t:
+            raise ValueError(f"a tensor with strides {t.stride()} cannot be turned in place together with the other one")
+        t = t.contiguous()
+        a = _layout(t, lead)
+    b = a if o is t else _layout(o, a[:2])
+    return t, (t.data_ptr(), o.data_ptr(), t.shape[-2], a[2], a[3], a[4], b[2], b[3], b[4]), a[:2]
+
+
+_NONE = (None, None, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, q, k, yq, yk):
+    """One launch for up to two tensors of equal leading dimensions; q or k may be None."""
+    ref, lead, aq, ak = q, None, _NONE, _NONE
+    if q is not None:
+        q, aq, lead = _args(q, yq, None)
+    else:
+        ref = k
+    if k is not None:
+        k, ak, lead = _args(k, yk, lead)
+    if positions.dim() != ref.dim() - 2 or positions.shape != ref.shape[:-2]:
         positions = positions.expand(ref.shape[:-2])
-    positions = positions.contiguous()
-    call_on(ref.device, "vamd_rotary", positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(), amplitude,
-            lead[0], lead[1], ref.shape[-1], turned, interleaved, inverse, *args, _TYPES[ref.dtype])
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    call_on(ref.device, "vamd_rotary", positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), amplitude,
+            lead[0], lead[1], ref.shape[-1], turned, interleaved, inverse, *aq, *ak, _TYPES[ref.dtype])
 
 
 def _readable(t):
-    return t if t is None or (t.stride(-1) == 1 and _rows(t) is not None) else t.contiguous()
+    return t if t is None or (t.stride(-1) == 1 and (t.dim() <= 4 or _layout(t) is not None)) else t.contiguous()
 
 
 def _fresh(x):
     """Memory for a result: x's own layout where it is dense and has few leading dimensions, else contiguous."""
+    if x is None:
+        return None
     y = torch.empty_like(x) if x.dim() <= 4 else None
     return y if y is not None and y.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _turned(positions, frequencies, how, q, k):
+    q, k = _readable(q), _readable(k)
+    yq, yk = _fresh(q), _fresh(k)
+    _turn(positions, frequencies, *how, q, k, yq, yk)
+    return yq, yk
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, positions, frequencies, amplitude, turned, interleaved, inverse, q, k):
+    def forward(ctx, positions, frequencies, how, q, k):
         ctx.save_for_backward(positions, frequencies)
-        ctx.how = (amplitude, turned, interleaved, inverse)
+        ctx.how = how
         ctx.set_materialize_grads(False)
-        xs = [_readable(q), _readable(k)]
-        outs = [None if x is None else _fresh(x) for x in xs]
-        _turn(positions, frequencies, amplitude, turned, interleaved, inverse, xs, outs)
-        return tuple(outs)
+        return _turned(positions, frequencies, how, q, k)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        positions, frequencies = ctx.saved_tensors
-        amplitude, turned, interleaved, inverse = ctx.how
-        if not ctx.needs_input_grad[6]:
+        if not ctx.needs_input_grad[3]:
             gq = None
-        if not ctx.needs_input_grad[7]:
+        if not ctx.needs_input_grad[4]:
             gk = None
         if gq is None and gk is None:
-            return (None,) * 8
+            return None, None, None, None, None
         # the transpose of a turn is the turn back, with the same amplitude: the same function, differentiable in turn
-        return (None,) * 6 + _RotaryFn.apply(positions, frequencies, amplitude, turned, interleaved, 1 - inverse, gq, gk)
+        turn = _RotaryFn.apply if torch.is_grad_enabled() else _turned
+        return (None, None, None) + tuple(turn(*ctx.saved_tensors, (*ctx.how[:3], 1 - ctx.how[3]), gq, gk))
 
 
 class Rotary(nn.Module):
@@ -151,6 +169,7 @@ class Rotary(nn.Module):
         turns = [round(Fraction(x) / (2 * _PI) * 2 ** 64) % 2 ** 64 for x in f]
         bits = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
         self.register_buffer("frequencies", bits, persistent=False)
+        self._how = (self.amplitude, rotary_dim, int(layout == "interleaved"), 0)
 
     def _check(self, positions, q, k):
         for name, t in (("q", q), ("k", k)):
@@ -180,13 +199,10 @@ class Rotary(nn.Module):
             if q.numel() == 0 and k.numel() == 0:
                 return q.clone(), k.clone()
             return (self(positions, q), k.clone()) if k.numel() == 0 else (q.clone(), self(positions, k))
-        how = (self.amplitude, self.rotary_dim, int(self.layout == "interleaved"), 0)
+        turn = _turned
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            yq, yk = _RotaryFn.apply(positions, self.frequencies, *how, q, k)
-        else:
-            xs = (_readable(q), _readable(k))
-            yq, yk = (None if x is None else _fresh(x) for x in xs)
-            _turn(positions, self.frequencies, *how, xs, (yq, yk))
+            turn = _RotaryFn.apply
+        yq, yk = turn(positions, self.frequencies, self._how, q, k)
         return yq if k is None else (yq, yk)
 
     def apply_(self, positions, q, k=None):
@@ -197,7 +213,7 @@ class Rotary(nn.Module):
                 continue
             if torch.is_grad_enabled() and t.requires_grad:
                 raise RuntimeError(f"{name} requires a gradient: apply_ is not differentiable, call the module instead")
-            if t.numel() and (t.stride(-1) != 1 or _rows(t) is None or self_overlapping(t)):
+            if t.numel() and (t.stride(-1) != 1 or _layout(t) is None or self_overlapping(t)):
                 raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
         if k is not None and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
             raise ValueError("q and k are the same memory")
@@ -208,5 +224,5 @@ class Rotary(nn.Module):
             if k is not None and (q.numel() or k.numel()):
                 self.apply_(positions, q if q.numel() else k)
             return q if k is None else (q, k)
-        _turn(positions, self.frequencies, self.amplitude, self.rotary_dim, int(self.layout == "interleaved"), 0, (q, k), (q, k))
+        _turn(positions, self.frequencies, *self._how, q, k, q, k)
         return q if k is None else (q, k)
