@@ -19,6 +19,8 @@
 // probabilities) give fp32 accuracy on the same matrix path.
 #include "kv_layout.h"
 
+#include <type_traits>
+
 namespace vamd {
 
 struct KvAttendArgs {
@@ -35,7 +37,7 @@ struct KvAttendArgs {
     float* part;                 // [tile rows][splits][D] outputs, then [tile rows][splits][2] maximum and sum
     float* part_ml;
     float scale2;                // scale * log2(e)
-    int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, splits, q_aligned, o_aligned;
+    int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, tile_rows, splits, q_aligned, o_aligned;
 };
 
 // Groups of 64 tokens that the rows of a tile can see: `sink_groups` from 0 on, then those from `first` on; `count` in all.
@@ -368,6 +370,319 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     }
 }
 
+#ifndef TILE_LB
+#define TILE_LB 2
+#endif
+// ---------------------------------------------------------------------------------------------------- many queries (prompts)
+//
+// A workgroup of four waves takes 128 * CB rows, a wave 32 * CB of them as the columns of v_mfma_f32_32x32x16_bf16, and walks over the
+// keys 64 at a time.  The codes of a group become bf16 ONCE per workgroup on their way into LDS (both operands in the
+// order in which the products read them, 16 bytes a lane, no bank conflicts; the next group's codes are in flight meanwhile and
+// go to the other buffer behind the products, one barrier a group).  A lane ends up with 16 scores of one query per 32 keys,
+// again in the slots in which the second product wants the probabilities: the row maximum needs one exchange between two lanes.
+// The running maximum is a reference that moves only when a score exceeds it by 2^8 or more (probabilities up to 256 are as exact
+// as below 1), so that the outputs are hardly ever rescaled.  The values' power-of-two scale goes into the exponent.
+//
+// DT: tiles of 32 features (the last may be half empty).
+__device__ __forceinline__ float kv_over_halves_max(float v) {               // over the two lanes that hold one query's keys
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float kv_over_halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+constexpr int kKvTileThreads = 256;
+
+template <typename T, int FMT, int DT, int CB>
+__global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel(const KvAttendArgs a) {
+    constexpr int N = sizeof(T) == 4 ? 3 : 1;
+    constexpr int PIECES = (DT * 2 * 64 + kKvTileThreads - 1) / kKvTileThreads;      // 16-byte pieces of a group a thread stages
+    constexpr int KBYTES = DT * 4 * 64 * 16, BUF = 2 * KBYTES;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, hh = lane >> 5;
+    // late tiles (the longest, where queries are causal) first; neighbouring workgroups take different heads, so that the tiles of one
+    // head meet in one XCD's L2 where the heads are a multiple of 8
+    uint32_t id = blockIdx.x;
+    const uint32_t pairs = (uint32_t)a.sequences * a.heads;
+    const uint32_t pair = id % pairs;
+    id /= pairs;
+    const int split = (int)(id % (uint32_t)a.splits), tile = a.tiles - 1 - (int)(id / (uint32_t)a.splits);
+    const int h = (int)(pair % (uint32_t)a.heads), b = (int)(pair / (uint32_t)a.heads);
+    const int64_t slot = ((int64_t)pair * a.tiles + tile) * a.tile_rows;
+
+    const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
+    const int all_rows = rows.count * a.group, first_row = tile * a.tile_rows;
+    if (first_row >= all_rows) return;
+    const int length = kv_length(a, b), shift = length - rows.count;
+    const int last_row = first_row + a.tile_rows - 1 < all_rows ? first_row + a.tile_rows - 1 : all_rows - 1;
+    const int p_first = a.causal ? shift + first_row / a.group : length - 1, p_last = a.causal ? shift + last_row / a.group : length - 1;
+    const KvRange range = kv_range(a, length, p_first, p_last);
+    const int per = kv_share(range.count, a.splits);
+    const int begin = split * per, end = begin + per < range.count ? begin + per : range.count;
+    if (split > 0 && begin >= range.count) return;
+    const int S = a.D >> 4;
+
+    auto group_of = [&](int x) { return x < range.sink_groups ? x : x - range.sink_groups + range.first; };
+    auto page_of = [&](int x) { return kv_page(a.table, a.table_stride, a.width, a.blocks, b, group_of(x) >> (a.block_shift - 6)); };
+    kv_u32x4 st[2][PIECES];                                                  // codes of the group after this one
+    float ks_next = 0.f, vs_next = 0.f;
+    int page_next = -1;
+    auto fetch = [&](int x) {
+        page_next = page_of(x);
+        const int64_t at = (int64_t)(page_next < 0 ? 0 : page_next) * a.heads + h;
+        const int64_t byte = ((at << a.block_shift) + (group_of(x) & ((1 << (a.block_shift - 6)) - 1)) * kKvGroup) * a.D;
+        ks_next = a.scales[0][at];
+        vs_next = a.scales[1][at];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int q = tid + i * kKvTileThreads;
+            if (q < 64 * S) {
+                st[0][i] = *((const kv_u32x4*)(a.codes[0] + byte) + q);
+                st[1][i] = *((const kv_u32x4*)(a.codes[1] + byte) + q);
+            }
+        }
+    };
+    // keys: [8 features][64 tokens]; values: [step of 16 tokens][half][feature], 8 tokens each (see above)
+    auto stage = [&](int buf) {
+        unsigned char* kb = smem + buf * BUF;
+        unsigned char* vb = kb + KBYTES;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int q = tid + i * kKvTileThreads;
+            if (q < 64 * S) {
+                const int token = (q >> 4) / S * 16 + (q & 15), slab = (q >> 4) % S;
+                *(kv_bf16x8*)(kb + ((slab * 2) * 64 + token) * 16) = kv_operand8<FMT>(st[0][i][0], st[0][i][1]);
+                *(kv_bf16x8*)(kb + ((slab * 2 + 1) * 64 + token) * 16) = kv_operand8<FMT>(st[0][i][2], st[0][i][3]);
+                const int g = (q >> 4) & 3, d = (q >> 6) * 16 + (q & 15);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const kv_bf16x8 w = kv_operand8<FMT>(st[1][i][2 * u], st[1][i][2 * u + 1]);
+                    const kv_u32x4 bits = __builtin_bit_cast(kv_u32x4, w);
+                    unsigned char* to = vb + (((4 * u + (g & 1)) * (DT * 32)) + d) * 16 + (g >> 1) * 8;
+                    *(kv_u32x2*)to = kv_u32x2{bits[0], bits[1]};
+                    *(kv_u32x2*)(to + 2 * (DT * 32) * 16) = kv_u32x2{bits[2], bits[3]};
+                }
+            }
+        }
+    };
+
+    if (begin < end) fetch(begin);
+    // queries: column c of block cb is row first_row + (wave * CB + cb) * 32 + c
+    kv_bf16x8 qf[CB][N][DT * 2];
+    int tok[CB], head[CB], upto[CB], from[CB];
+    bool live[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        const int row = first_row + (wave * CB + cb) * 32 + c;
+        tok[cb] = row / a.group;
+        head[cb] = h * a.group + row - tok[cb] * a.group;
+        live[cb] = tok[cb] < rows.count;
+        const int pos = a.causal ? shift + tok[cb] : length - 1;
+        upto[cb] = pos < length ? pos : length - 1;
+        from[cb] = a.window > 0 ? pos - a.window + 1 : 0;
+        const T* q = (const T*)a.q + (rows.first + (live[cb] ? tok[cb] : 0)) * a.q_tok + head[cb] * a.q_head;
+#pragma unroll
+        for (int k = 0; k < DT * 2; ++k) {
+            T v[8] = {};
+            if (live[cb] && k < S) {
+                const T* p = q + k * 16 + hh * 8;
+                if (a.q_aligned) {
+#pragma unroll
+                    for (int i = 0; i < 8 / Vec16<T>::N; ++i) *(Vec16<T>*)(v + i * Vec16<T>::N) = *(const Vec16<T>*)(p + i * Vec16<T>::N);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = p[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (N == 1) qf[cb][0][k][e] = v[e];
+                else {
+                    bf16_t p[N];
+                    kv_pieces<N>(v[e], p);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) qf[cb][n][k][e] = p[n];
+                }
+            }
+        }
+    }
+    const int first_keys = a.window > 0 ? a.sinks : 0;
+    kv_f32x16 acc[CB][DT];
+    float m[CB], l[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        m[cb] = -INFINITY;
+        l[cb] = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[cb][t][i] = 0.f;
+    }
+    if (begin < end) stage(0);
+    int buf = 0;
+    for (int x = begin; x < end; ++x, buf ^= 1) {
+        const float f_raw = a.scale2 * ks_next, v_scale = vs_next;
+        const int page = page_next, k0 = group_of(x) * kKvGroup;
+        const bool more = x + 1 < end;
+        __syncthreads();                                     // this buffer is written, the other one read
+        if (more) fetch(x + 1);
+        const unsigned char* kb = smem + buf * BUF;
+        const unsigned char* vb = kb + KBYTES;
+        kv_f32x16 sc[CB][2];
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[cb][kh][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < DT * 2; ++k) {
+                if (k < S) {
+                    const kv_bf16x8 kf = *(const kv_bf16x8*)(kb + ((k * 2 + hh) * 64 + kh * 32 + c) * 16);
+#pragma unroll
+                    for (int n = N - 1; n >= 0; --n)
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb)
+                            sc[cb][kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[cb][n][k], sc[cb][kh], 0, 0, 0);
+                }
+            }
+        }
+        // scores stay unscaled until the exponential; a hidden one is an infinity that f turns into -inf (f = 0: no infinity must meet it)
+        const bool by_hand = !(fabsf(f_raw) > 0.f && fabsf(f_raw) < INFINITY);
+        const float f = by_hand ? 1.f : f_raw;
+        if (by_hand) {
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[cb][kh][i] *= f_raw;
+        }
+        const float hidden = f < 0.f ? INFINITY : -INFINITY;
+        const bool edge = page < 0 || k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
+                          (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
+        // 2^e = v_scale is added to the exponents unless it is so far from 1 that probabilities could leave the range of a float
+        const int v_exp = (int)(__float_as_uint(v_scale) >> 23) - 127;
+        const bool fold = v_exp >= -40 && v_exp <= 40;
+        const float v_add = fold ? (float)v_exp : 0.f, v_undo = fold ? __uint_as_float((uint32_t)(127 - v_exp) << 23) : 1.f;
+        kv_bf16x8 pf[CB][N][4];
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if (edge) {
+                const int k1 = k0 + hh * 4;
+                const int rel_upto = page < 0 ? -1 : upto[cb] - k1, rel_from = from[cb] - k1, rel_first = first_keys - k1;
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = kh * 32 + (i >> 2) * 8 + (i & 3);
+                        const bool seen = j <= rel_upto && (j >= rel_from || j < rel_first);
+                        sc[cb][kh][i] = seen ? sc[cb][kh][i] : hidden;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[cb][kh][i] * f);
+            top = kv_over_halves_max(top);
+            if (__any(top > m[cb] + 8.f)) {
+                const float m_new = top > m[cb] + 8.f ? top : m[cb];
+                const float alpha = __builtin_amdgcn_exp2f(m[cb] - kv_finite(m_new));
+                l[cb] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[cb][t][i] *= alpha;
+                m[cb] = m_new;
+            }
+            const float shift_by = v_add - kv_finite(m[cb]);
+            float sum = 0.f;
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[cb][kh][i], f, shift_by));
+                    sum += e;
+                    sc[cb][kh][i] = e;
+                }
+            l[cb] = fmaf(sum, v_undo, l[cb]);
+            if (!fold) {                                     // NaN: only to the queries that see the block
+#pragma unroll
+                for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = k0 + hh * 4 + kh * 32 + (i >> 2) * 8 + (i & 3);
+                        const bool seen = page >= 0 && j <= upto[cb] && (j >= from[cb] || j < first_keys);
+                        sc[cb][kh][i] = seen ? sc[cb][kh][i] * v_scale : 0.f;
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    bf16_t p[N];
+                    kv_pieces<N>(sc[cb][s >> 1][(s & 1) * 8 + e], p);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) pf[cb][n][s][e] = p[n];
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const kv_bf16x8 vf = *(const kv_bf16x8*)(vb + ((s * 2 + hh) * (DT * 32) + t * 32 + c) * 16);
+#pragma unroll
+                for (int n = N - 1; n >= 0; --n)
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb) acc[cb][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[cb][n][s], acc[cb][t], 0, 0, 0);
+            }
+        if (more) stage(buf ^ 1);
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        const float total = kv_over_halves_sum(l[cb]);
+        if (!live[cb]) continue;
+        if (a.splits > 1) {
+            const int64_t at = (slot + (wave * CB + cb) * 32 + c) * a.splits + split;
+            float* part = a.part + at * a.D;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t * 2 + (i >> 1) < S)
+                        *(kv_f32x4*)(part + t * 32 + i * 8 + hh * 4) = kv_f32x4{acc[cb][t][4 * i], acc[cb][t][4 * i + 1], acc[cb][t][4 * i + 2], acc[cb][t][4 * i + 3]};
+            if (hh == 0) {
+                a.part_ml[at * 2] = m[cb];
+                a.part_ml[at * 2 + 1] = total;
+            }
+            continue;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        T* o = (T*)a.o + (rows.first + tok[cb]) * a.o_tok + head[cb] * a.o_head;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t * 2 + (i >> 1) >= S) continue;
+                T v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = from_f<T>(acc[cb][t][4 * i + e] * inv);
+                T* to = o + t * 32 + i * 8 + hh * 4;
+                if (a.o_aligned) {
+                    if (sizeof(T) == 4) *(kv_u32x4*)to = *(const kv_u32x4*)v;
+                    else *(kv_u32x2*)to = *(const kv_u32x2*)v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[e] = v[e];
+                }
+            }
+    }
+}
+
 // Joins the shares of a row: one workgroup of 16 waves per row.  The shares' weights go to LDS first, so that the loads of the
 // outputs depend on nothing; a lane then reads four features of every (1024 / lanes a row takes)-th share, eight in flight.
 constexpr int kKvMaxSplits = 256;
@@ -380,13 +695,13 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     const uint32_t per_head = (uint32_t)a.most * a.group;
     const int row = (int)(id % per_head);
     id /= per_head;
-    const int64_t slot = (int64_t)id * a.tiles * 16 + row;
+    const int64_t slot = (int64_t)id * a.tiles * a.tile_rows + row;
     const int h = (int)(id % (uint32_t)a.heads), b = (int)(id / (uint32_t)a.heads);
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int tok = row / a.group;
     if (tok >= rows.count) return;
-    const int length = kv_length(a, b), shift = length - rows.count, r0 = row & ~15;
-    const int r1 = r0 + 15 < rows.count * a.group ? r0 + 15 : rows.count * a.group - 1;
+    const int length = kv_length(a, b), shift = length - rows.count, r0 = row / a.tile_rows * a.tile_rows;
+    const int r1 = r0 + a.tile_rows < rows.count * a.group ? r0 + a.tile_rows - 1 : rows.count * a.group - 1;
     const KvRange range = kv_range(a, length, a.causal ? shift + r0 / a.group : length - 1, a.causal ? shift + r1 / a.group : length - 1);
     const int per = kv_share(range.count, a.splits);
     int used = (range.count + per - 1) / per;
@@ -436,18 +751,29 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     }
 }
 
+#ifndef CBV
+#define CBV 1
+#define TILE_LB 2
+#endif
+static int kv_tile_rows(int64_t rows, int dim, int dtype) {
+    if (rows <= 64 || (dtype == VAMD_F32 && dim > 128)) return 16;
+    return 128 * CBV;
+}
+
 // How a call is cut: tiles of 16 rows of a (sequence, key head), and shares of the keys so that 512 workgroups (two a CU, all
 // resident) have work, none of them less than 8 groups of 64 tokens.  One token of 64 sequences of up to 4096 (8 key heads, 128
 // features): 61 us with 256 or 512, 65 with 768, 79 with 1024 workgroups; of one sequence of 131071: 40, 42, 47 and 46 us.
 struct KvPlan {
-    int tiles, splits;
+    int tile_rows, tiles, splits;
     int64_t slots;
 };
-static KvPlan kv_plan(int sequences, int most, int64_t longest, int heads, int group) {
+static KvPlan kv_plan(int sequences, int most, int64_t longest, int heads, int group, int dim, int dtype) {
     KvPlan p;
-    p.tiles = (int)(((int64_t)most * group + 15) / 16);
+    const int64_t rows = (int64_t)most * group;
+    p.tile_rows = kv_tile_rows(rows, dim, dtype);
+    p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     const int64_t base = (int64_t)sequences * heads * p.tiles;
-    p.slots = base * 16;
+    p.slots = base * p.tile_rows;
     const int64_t groups = (longest + kKvGroup - 1) / kKvGroup;
     int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
     if (splits > (groups + kKvMinShare - 1) / kKvMinShare) splits = (groups + kKvMinShare - 1) / kKvMinShare;
@@ -471,6 +797,34 @@ template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, 
     return 0;
 }
 
+template <typename T, int FMT, int DT> static int kv_launch_tile_of(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
+    constexpr int LDS = 2 * 2 * DT * 4 * 64 * 16;
+    auto kernel = kv_attend_tile_kernel<T, FMT, DT, CBV>;
+    if (LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return fail((int)e, "vamd_kv_attend: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kKvTileThreads), LDS, st, a);
+    VAMD_LAUNCH_OK("kv_attend_tile");
+    return 0;
+}
+template <typename T, int FMT> static int kv_launch_tile(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
+    switch ((a.D + 31) / 32) {
+        case 1: return kv_launch_tile_of<T, FMT, 1>(a, grid, st);
+        case 2: return kv_launch_tile_of<T, FMT, 2>(a, grid, st);
+        case 3: return kv_launch_tile_of<T, FMT, 3>(a, grid, st);
+        case 4: return kv_launch_tile_of<T, FMT, 4>(a, grid, st);
+    }
+    if constexpr (sizeof(T) == 2) {
+        switch ((a.D + 31) / 32) {
+            case 5:
+            case 6: return kv_launch_tile_of<T, FMT, 6>(a, grid, st);
+            default: return kv_launch_tile_of<T, FMT, 8>(a, grid, st);
+        }
+    }
+    return fail(VAMD_EUNSUPPORTED, "vamd_kv_attend: no kernel for %d features in float32", a.D);
+}
+
 // One wave per row, four or sixteen: so many that a lane reads about four shares.  32 rows of 256 shares: 12 us with four waves, 5.8 with
 // sixteen; 512 rows of 4 shares (128 features): 18 us with sixteen waves, 4 with one.
 template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream_t st) {
@@ -487,9 +841,9 @@ template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream
 
 using namespace vamd;
 
-extern "C" size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim) {
+extern "C" size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim, int dtype) {
     if (sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
-    const KvPlan p = kv_plan(sequences, most, longest, heads, group);
+    const KvPlan p = kv_plan(sequences, most, longest, heads, group, dim, dtype);
     return p.splits > 1 ? (size_t)p.slots * p.splits * (dim + 2) * sizeof(float) : 0;
 }
 
@@ -518,11 +872,11 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE((uintptr_t)codes_k % 16 == 0 && (uintptr_t)codes_v % 16 == 0 && (uintptr_t)scales_k % 4 == 0 && (uintptr_t)scales_v % 4 == 0 &&
                  (uintptr_t)table % 4 == 0 && (uintptr_t)lengths % 4 == 0 && (uintptr_t)offsets % 4 == 0 && (uintptr_t)q % size == 0 &&
                  (uintptr_t)o % size == 0, "vamd_kv_attend: misaligned tensor");
-    const KvPlan plan = kv_plan(sequences, most, longest, heads, group);
-    const size_t need = vamd_kv_attend_workspace(sequences, most, longest, heads, group, dim);
+    const KvPlan plan = kv_plan(sequences, most, longest, heads, group, dim, dtype);
+    const size_t need = vamd_kv_attend_workspace(sequences, most, longest, heads, group, dim, dtype);
     VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                  "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    const int64_t grid = plan.slots / 16 * plan.splits;
+    const int64_t grid = plan.slots / plan.tile_rows * plan.splits;
     VAMD_REQUIRE(grid <= 0x7fffffff && plan.slots <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
                  sequences, most);
     KvAttendArgs a = {};
@@ -556,14 +910,22 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     a.sinks = sinks;
     a.causal = causal;
     a.tiles = plan.tiles;
+    a.tile_rows = plan.tile_rows;
     a.splits = plan.splits;
     const int n = 16 / size;
     a.q_aligned = (uintptr_t)q % 16 == 0 && q_token % n == 0 && q_head % n == 0;
     a.o_aligned = (uintptr_t)o % (4 * size) == 0 && o_token % 4 == 0 && o_head % 4 == 0;
     hipStream_t st = as_stream(stream);
+    auto launch = [&](auto t, auto f) {
+        using T = decltype(t);
+        constexpr int FMT = decltype(f)::value;
+        return plan.tile_rows == 16 ? kv_launch_rows<T, FMT>(a, grid, st) : kv_launch_tile<T, FMT>(a, grid, st);
+    };
+    const std::integral_constant<int, VAMD_KV_E4M3> e4m3;
+    const std::integral_constant<int, VAMD_KV_INT8> int8;
     int rc;
-    if (dtype == VAMD_BF16) rc = format == VAMD_KV_E4M3 ? kv_launch_rows<bf16_t, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<bf16_t, VAMD_KV_INT8>(a, grid, st);
-    else rc = format == VAMD_KV_E4M3 ? kv_launch_rows<float, VAMD_KV_E4M3>(a, grid, st) : kv_launch_rows<float, VAMD_KV_INT8>(a, grid, st);
+    if (dtype == VAMD_BF16) rc = format == VAMD_KV_E4M3 ? launch(bf16_t(), e4m3) : launch(bf16_t(), int8);
+    else rc = format == VAMD_KV_E4M3 ? launch(float(), e4m3) : launch(float(), int8);
     if (rc || plan.splits == 1) return rc;
     return dtype == VAMD_BF16 ? kv_launch_join<bf16_t>(a, st) : kv_launch_join<float>(a, st);
 }

@@ -150,7 +150,7 @@ class KVCache:
         room = width * self.block
         longest = room if longest is None else min(max(int(longest), 0), room)
         group = heads // self.kv_heads
-        size = lib.vamd_kv_attend_workspace(n, most, longest, self.kv_heads, group, self.head_dim)
+        size = lib.vamd_kv_attend_workspace(n, most, longest, self.kv_heads, group, self.head_dim, _TYPES[q.dtype])
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         qs, os = q.stride(), out.stride()
         call_on(self.device, "vamd_kv_attend", q.data_ptr(), qs[0], qs[1], *self._pointers, table.data_ptr(), table.stride(0),
