@@ -542,7 +542,8 @@ int vamd_kv_read(const void* codes_k, const void* codes_v, const float* scales_k
  * keys up to its position, with window > 0 only the last `window` of them and the first `sinks`; else all.  Tokens in
  * holes are not seen; a query that sees nothing gives zeros.  `longest` (a bound of the lengths) only steers how the work is
  * cut.  workspace: vamd_kv_attend_workspace bytes (may be 0), 16-byte aligned. */
-size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim, int dtype);
+size_t vamd_kv_attend_workspace(int64_t rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window,
+                                int sinks, int dtype);
 int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, const void* codes_k, const void* codes_v,
                    const float* scales_k, const float* scales_v, const int32_t* table, int64_t table_stride,
                    const int32_t* lengths, const int32_t* offsets, int64_t rows, int sequences, int most, int64_t longest,

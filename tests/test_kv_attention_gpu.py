@@ -117,7 +117,7 @@ def test_long_contexts_split_and_joined(format, dtype):
     lengths = [20000, 513, 6001]
     c, table, k, v, off = filled(lengths, 1, 128, 128, format, 60)
     q = rnd((3, 4, 128), dtype, 69)
-    assert lib.vamd_kv_attend_workspace(3, 1, 20000, 1, 4, 128, _lib.BF16) > 0
+    assert lib.vamd_kv_attend_workspace(3, 3, 1, 20000, 1, 4, 128, 0, 0, _lib.BF16) > 0
     out = c.attend(q, table, i32(lengths), longest=20000)
     compare(out, q, k, v, off, lengths, [1, 1, 1], 128 ** -0.5, dtype)
     # the bound steers the split only: too low, or far too high, the result is right

@@ -225,7 +225,7 @@ def test_attend_entry_refuses(bad):
 
 def test_attend_entry_with_nothing_to_do():
     assert attend_call(rows=0, most=0) == 0
-    assert lib.vamd_kv_attend_workspace(0, 1, 64, 1, 1, 64, 0) == 0
+    assert lib.vamd_kv_attend_workspace(1, 0, 1, 64, 1, 1, 64, 0, 0, 0) == 0
 
 
 # ---------------------------------------------------------------------------------------------------- index functions, on the host

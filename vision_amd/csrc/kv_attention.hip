@@ -59,10 +59,11 @@ __device__ __forceinline__ KvRange kv_range(const KvAttendArgs& a, int length, i
     return KvRange{sink, first, sink + last - first};
 }
 // The share of a split: at least 8 groups, so that short sequences of a batch do not fall into crumbs.
-constexpr int kKvMinShare = 8;
-__device__ __forceinline__ int kv_share(int count, int splits) {
-    const int per = (count + splits - 1) / splits;
-    return per < kKvMinShare ? kKvMinShare : per;
+// (tiles of many rows: 16 groups, because joining their rows costs more)
+__host__ __device__ constexpr int kv_min_share(int tile_rows) { return tile_rows > 16 ? 16 : 8; }
+__device__ __forceinline__ int kv_share(int count, int splits, int tile_rows) {
+    const int per = (count + splits - 1) / splits, least = kv_min_share(tile_rows);
+    return per < least ? least : per;
 }
 __device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
     const int64_t room = (int64_t)a.width << a.block_shift;
@@ -104,13 +105,14 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
+    // heads and sequences vary fastest, shares slowest: workgroups without work (shares that a short sequence does not have) then
+    // sit behind each other and not on every second XCD or CU
     uint32_t id = blockIdx.x;
-    const int split = (int)(id % (uint32_t)a.splits);
-    id /= (uint32_t)a.splits;
-    const int64_t slot = (int64_t)id * 16;
-    const int tile = (int)(id % (uint32_t)a.tiles);
-    id /= (uint32_t)a.tiles;
-    const int h = (int)(id % (uint32_t)a.heads), b = (int)(id / (uint32_t)a.heads);
+    const uint32_t pairs = (uint32_t)a.sequences * a.heads, pair = id % pairs;
+    id /= pairs;
+    const int tile = (int)(id % (uint32_t)a.tiles), split = (int)(id / (uint32_t)a.tiles);
+    const int h = (int)(pair % (uint32_t)a.heads), b = (int)(pair / (uint32_t)a.heads);
+    const int64_t slot = ((int64_t)pair * a.tiles + tile) * 16;
 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     if (tile * 16 >= rows.count * a.group) return;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     last_row = last_row < rows.count * a.group ? last_row : rows.count * a.group - 1;
     const int p_first = a.causal ? shift + tile * 16 / a.group : length - 1, p_last = a.causal ? shift + last_row / a.group : length - 1;
     const KvRange range = kv_range(a, length, p_first, p_last);
-    const int per = kv_share(range.count, a.splits);
+    const int per = kv_share(range.count, a.splits, a.tile_rows);
     const int begin = split * per, end = begin + per < range.count ? begin + per : range.count;
     if (split > 0 && begin >= range.count) return;
 
@@ -370,9 +372,6 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     }
 }
 
-#ifndef TILE_LB
-#define TILE_LB 2
-#endif
 // ---------------------------------------------------------------------------------------------------- many queries (prompts)
 //
 // A workgroup of four waves takes 128 * CB rows, a wave 32 * CB of them as the columns of v_mfma_f32_32x32x16_bf16, and walks over the
@@ -393,49 +392,85 @@ __device__ __forceinline__ float kv_over_halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr int kKvTileThreads = 256;
+constexpr int kKvTileThreads = 256, kKvTileRows = 128;
 
 template <typename T, int FMT, int DT, int CB>
-__global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4) ? 2 : 1) kv_attend_tile_kernel(const KvAttendArgs a) {
     constexpr int N = sizeof(T) == 4 ? 3 : 1;
     constexpr int PIECES = (DT * 2 * 64 + kKvTileThreads - 1) / kKvTileThreads;      // 16-byte pieces of a group a thread stages
     constexpr int KBYTES = DT * 4 * 64 * 16, BUF = 2 * KBYTES;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, hh = lane >> 5;
-    // late tiles (the longest, where queries are causal) first; neighbouring workgroups take different heads, so that the tiles of one
-    // head meet in one XCD's L2 where the heads are a multiple of 8
+    // Heads vary fastest (where they are a multiple of 8 the tiles of one meet in one XCD's L2), then the shares, then the tiles that
+    // the sequences really have, one sequence after the other, late ones (the longest, where queries are causal) first.  Walked over by
+    // `most` instead, tiles that short sequences do not have lie between the others in a regular pattern that leaves whole
+    // CUs idle: prompts of 4096 and 925 tokens 435 us, of 4096 alone 264.
     uint32_t id = blockIdx.x;
-    const uint32_t pairs = (uint32_t)a.sequences * a.heads;
-    const uint32_t pair = id % pairs;
-    id /= pairs;
-    const int split = (int)(id % (uint32_t)a.splits), tile = a.tiles - 1 - (int)(id / (uint32_t)a.splits);
-    const int h = (int)(pair % (uint32_t)a.heads), b = (int)(pair / (uint32_t)a.heads);
-    const int64_t slot = ((int64_t)pair * a.tiles + tile) * a.tile_rows;
-
+    const int h = (int)(id % (uint32_t)a.heads);
+    id /= (uint32_t)a.heads;
+    const int split = (int)(id % (uint32_t)a.splits);
+    int tile = (int)(id / (uint32_t)a.splits), b = 0;
+    if (!a.offsets) {
+        b = tile / a.tiles;
+        tile -= b * a.tiles;
+    } else {
+        for (int b0 = 0;; b0 += 64) {                        // 64 sequences at a time: whose tile is it?
+            if (b0 >= a.sequences) return;
+            const int mine = b0 + lane;
+            int n = 0;
+            if (mine < a.sequences) n = (kv_rows(a.offsets, mine, a.rows, a.most).count * a.group + a.tile_rows - 1) / a.tile_rows;
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int t = __shfl_up(upto, o, 64);
+                upto += lane >= o ? t : 0;
+            }
+            const uint64_t behind = __ballot(upto > tile);
+            if (behind) {
+                const int l = __ffsll((unsigned long long)behind) - 1;
+                b = b0 + l;
+                tile -= __shfl(upto - n, l, 64);
+                break;
+            }
+            tile -= __shfl(upto, 63, 64);
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        tile = __builtin_amdgcn_readfirstlane(tile);
+    }
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
-    const int all_rows = rows.count * a.group, first_row = tile * a.tile_rows;
-    if (first_row >= all_rows) return;
+    const int all_rows = rows.count * a.group;
+    tile = (all_rows + a.tile_rows - 1) / a.tile_rows - 1 - tile;
+    if (tile < 0) return;
+    const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * a.tile_rows;
+    const int first_row = tile * a.tile_rows;
     const int length = kv_length(a, b), shift = length - rows.count;
     const int last_row = first_row + a.tile_rows - 1 < all_rows ? first_row + a.tile_rows - 1 : all_rows - 1;
     const int p_first = a.causal ? shift + first_row / a.group : length - 1, p_last = a.causal ? shift + last_row / a.group : length - 1;
     const KvRange range = kv_range(a, length, p_first, p_last);
-    const int per = kv_share(range.count, a.splits);
+    const int per = kv_share(range.count, a.splits, a.tile_rows);
     const int begin = split * per, end = begin + per < range.count ? begin + per : range.count;
     if (split > 0 && begin >= range.count) return;
     const int S = a.D >> 4;
 
     auto group_of = [&](int x) { return x < range.sink_groups ? x : x - range.sink_groups + range.first; };
-    auto page_of = [&](int x) { return kv_page(a.table, a.table_stride, a.width, a.blocks, b, group_of(x) >> (a.block_shift - 6)); };
+    // The table's entries and the scales come through vector loads (an address that depends on a register): a scalar load in
+    // flight makes every wait for LDS a wait for all of it.  Entries are loaded two groups ahead.
+    int lane_zero;
+    asm volatile("v_mov_b32 %0, 0" : "=v"(lane_zero));
+    const int32_t* entries = a.table + b * a.table_stride + lane_zero;
+    auto entry_of = [&](int x) {                             // length <= width blocks: never behind the table's row
+        x = x < end ? x : end - 1;
+        return entries[group_of(x) >> (a.block_shift - 6)];
+    };
     kv_u32x4 st[2][PIECES];                                                  // codes of the group after this one
     float ks_next = 0.f, vs_next = 0.f;
-    int page_next = -1;
+    int page_next = -1, entry = -1;
     auto fetch = [&](int x) {
-        page_next = page_of(x);
+        page_next = __builtin_amdgcn_readfirstlane(entry);
+        if (page_next >= a.blocks) page_next = -1;           // a hole, as a negative entry is
         const int64_t at = (int64_t)(page_next < 0 ? 0 : page_next) * a.heads + h;
         const int64_t byte = ((at << a.block_shift) + (group_of(x) & ((1 << (a.block_shift - 6)) - 1)) * kKvGroup) * a.D;
-        ks_next = a.scales[0][at];
-        vs_next = a.scales[1][at];
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int q = tid + i * kKvTileThreads;
@@ -444,6 +479,9 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
                 st[1][i] = *((const kv_u32x4*)(a.codes[1] + byte) + q);
             }
         }
+        ks_next = (a.scales[0] + at)[lane_zero];
+        vs_next = (a.scales[1] + at)[lane_zero];
+        entry = entry_of(x + 1);
     };
     // keys: [8 features][64 tokens]; values: [step of 16 tokens][half][feature], 8 tokens each (see above)
     auto stage = [&](int buf) {
@@ -454,22 +492,29 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
             const int q = tid + i * kKvTileThreads;
             if (q < 64 * S) {
                 const int token = (q >> 4) / S * 16 + (q & 15), slab = (q >> 4) % S;
-                *(kv_bf16x8*)(kb + ((slab * 2) * 64 + token) * 16) = kv_operand8<FMT>(st[0][i][0], st[0][i][1]);
-                *(kv_bf16x8*)(kb + ((slab * 2 + 1) * 64 + token) * 16) = kv_operand8<FMT>(st[0][i][2], st[0][i][3]);
+                const kv_u32x4 kw = kv_as_loaded(st[0][i]);
+                *(kv_bf16x8*)(kb + ((slab * 2) * 64 + token) * 16) = kv_operand8<FMT>(kw[0], kw[1]);
+                *(kv_bf16x8*)(kb + ((slab * 2 + 1) * 64 + token) * 16) = kv_operand8<FMT>(kw[2], kw[3]);
+                if (FMT == VAMD_KV_INT8) __builtin_amdgcn_sched_barrier(0);  // one conversion's floats at a time
                 const int g = (q >> 4) & 3, d = (q >> 6) * 16 + (q & 15);
+                const kv_u32x4 vw = kv_as_loaded(st[1][i]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const kv_bf16x8 w = kv_operand8<FMT>(st[1][i][2 * u], st[1][i][2 * u + 1]);
+                    const kv_bf16x8 w = kv_operand8<FMT>(vw[2 * u], vw[2 * u + 1]);
                     const kv_u32x4 bits = __builtin_bit_cast(kv_u32x4, w);
                     unsigned char* to = vb + (((4 * u + (g & 1)) * (DT * 32)) + d) * 16 + (g >> 1) * 8;
                     *(kv_u32x2*)to = kv_u32x2{bits[0], bits[1]};
                     *(kv_u32x2*)(to + 2 * (DT * 32) * 16) = kv_u32x2{bits[2], bits[3]};
+                    if (FMT == VAMD_KV_INT8) __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
     };
 
-    if (begin < end) fetch(begin);
+    if (begin < end) {
+        entry = entry_of(begin);
+        fetch(begin);
+    }
     // queries: column c of block cb is row first_row + (wave * CB + cb) * 32 + c
     kv_bf16x8 qf[CB][N][DT * 2];
     int tok[CB], head[CB], upto[CB], from[CB];
@@ -521,37 +566,66 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[cb][t][i] = 0.f;
     }
-    if (begin < end) stage(0);
+    if (begin < end) {
+        // keys' slabs that the head does not have are zero in both buffers (values' rows there end up in outputs that nobody reads)
+        for (int q = S * 128 + tid; q < DT * 2 * 128; q += kKvTileThreads) {
+            *(kv_u32x4*)(smem + q * 16) = kv_u32x4{0, 0, 0, 0};
+            *(kv_u32x4*)(smem + BUF + q * 16) = kv_u32x4{0, 0, 0, 0};
+        }
+        stage(0);
+    }
     int buf = 0;
     for (int x = begin; x < end; ++x, buf ^= 1) {
-        const float f_raw = a.scale2 * ks_next, v_scale = vs_next;
+        const float f_raw = a.scale2 * __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ks_next)));
+        const float v_scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(vs_next)));
         const int page = page_next, k0 = group_of(x) * kKvGroup;
         const bool more = x + 1 < end;
         __syncthreads();                                     // this buffer is written, the other one read
         if (more) fetch(x + 1);
         const unsigned char* kb = smem + buf * BUF;
         const unsigned char* vb = kb + KBYTES;
+        // operands are read in batches of R, one batch ahead of the products
+        constexpr int R = DT % 2 ? 2 : 4, BATCHES = DT * 4 / R;
+        kv_bf16x8 fr[2][R];
+        auto read_k = [&](int i) {                           // batch i: keys 32 kh + c, features 16 k + 8 hh ..
+#pragma unroll
+            for (int e = 0; e < R; ++e) {
+                const int kh = (i * R + e) / (DT * 2), k = (i * R + e) % (DT * 2);
+                fr[i & 1][e] = *(const kv_bf16x8*)(kb + ((k * 2 + hh) * 64 + kh * 32 + c) * 16);
+            }
+        };
+        auto read_v = [&](int i) {                           // batch i: feature 32 t + c, tokens of step s and half hh
+#pragma unroll
+            for (int e = 0; e < R; ++e) {
+                const int s = (i * R + e) / DT, t = (i * R + e) % DT;
+                fr[i & 1][e] = *(const kv_bf16x8*)(vb + ((s * 2 + hh) * (DT * 32) + t * 32 + c) * 16);
+            }
+        };
         kv_f32x16 sc[CB][2];
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
+        for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[cb][kh][i] = 0.f;
+        read_k(0);
 #pragma unroll
-            for (int k = 0; k < DT * 2; ++k) {
-                if (k < S) {
-                    const kv_bf16x8 kf = *(const kv_bf16x8*)(kb + ((k * 2 + hh) * 64 + kh * 32 + c) * 16);
+        for (int i = 0; i < BATCHES; ++i) {
+            if (i + 1 < BATCHES) read_k(i + 1);
 #pragma unroll
-                    for (int n = N - 1; n >= 0; --n)
+            for (int e = 0; e < R; ++e) {
+                const int kh = (i * R + e) / (DT * 2), k = (i * R + e) % (DT * 2);
 #pragma unroll
-                        for (int cb = 0; cb < CB; ++cb)
-                            sc[cb][kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[cb][n][k], sc[cb][kh], 0, 0, 0);
-                }
+                for (int n = N - 1; n >= 0; --n)
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb)
+                        sc[cb][kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], qf[cb][n][k], sc[cb][kh], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // scores stay unscaled until the exponential; a hidden one is an infinity that f turns into -inf (f = 0: no infinity must meet it)
-        const bool by_hand = !(fabsf(f_raw) > 0.f && fabsf(f_raw) < INFINITY);
+        read_v(0);                                           // in flight during the softmax
+        // scores stay unscaled until the exponential, which takes a positive factor; any other one (negative, 0, NaN) is applied here
+        const bool by_hand = !(f_raw > 0.f && f_raw < INFINITY);
         const float f = by_hand ? 1.f : f_raw;
         if (by_hand) {
 #pragma unroll
@@ -561,7 +635,6 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sc[cb][kh][i] *= f_raw;
         }
-        const float hidden = f < 0.f ? INFINITY : -INFINITY;
         const bool edge = page < 0 || k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
                           (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
         // 2^e = v_scale is added to the exponents unless it is so far from 1 that probabilities could leave the range of a float
@@ -580,15 +653,15 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
                     for (int i = 0; i < 16; ++i) {
                         const int j = kh * 32 + (i >> 2) * 8 + (i & 3);
                         const bool seen = j <= rel_upto && (j >= rel_from || j < rel_first);
-                        sc[cb][kh][i] = seen ? sc[cb][kh][i] : hidden;
+                        sc[cb][kh][i] = seen ? sc[cb][kh][i] : -INFINITY;
                     }
             }
             float top = -INFINITY;
 #pragma unroll
             for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[cb][kh][i] * f);
-            top = kv_over_halves_max(top);
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[cb][kh][i]);
+            top = kv_over_halves_max(top) * f;
             if (__any(top > m[cb] + 8.f)) {
                 const float m_new = top > m[cb] + 8.f ? top : m[cb];
                 const float alpha = __builtin_amdgcn_exp2f(m[cb] - kv_finite(m_new));
@@ -631,15 +704,19 @@ __global__ void __launch_bounds__(kKvTileThreads, TILE_LB) kv_attend_tile_kernel
                 }
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int i = 0; i < BATCHES; ++i) {
+            if (i + 1 < BATCHES) read_v(i + 1);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const kv_bf16x8 vf = *(const kv_bf16x8*)(vb + ((s * 2 + hh) * (DT * 32) + t * 32 + c) * 16);
+            for (int e = 0; e < R; ++e) {
+                const int s = (i * R + e) / DT, t = (i * R + e) % DT;
 #pragma unroll
                 for (int n = N - 1; n >= 0; --n)
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) acc[cb][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[cb][n][s], acc[cb][t], 0, 0, 0);
+                    for (int cb = 0; cb < CB; ++cb)
+                        acc[cb][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], pf[cb][n][s], acc[cb][t], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (more) stage(buf ^ 1);
     }
 #pragma unroll
@@ -703,7 +780,7 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     const int length = kv_length(a, b), shift = length - rows.count, r0 = row / a.tile_rows * a.tile_rows;
     const int r1 = r0 + a.tile_rows < rows.count * a.group ? r0 + a.tile_rows - 1 : rows.count * a.group - 1;
     const KvRange range = kv_range(a, length, a.causal ? shift + r0 / a.group : length - 1, a.causal ? shift + r1 / a.group : length - 1);
-    const int per = kv_share(range.count, a.splits);
+    const int per = kv_share(range.count, a.splits, a.tile_rows);
     int used = (range.count + per - 1) / per;
     used = used < 1 ? 1 : used;
     const float* ml = a.part_ml + slot * a.splits * 2;
@@ -751,33 +828,42 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     }
 }
 
-#ifndef CBV
-#define CBV 1
-#define TILE_LB 2
-#endif
-static int kv_tile_rows(int64_t rows, int dim, int dtype) {
-    if (rows <= 64 || (dtype == VAMD_F32 && dim > 128)) return 16;
-    return 128 * CBV;
-}
-
-// How a call is cut: tiles of 16 rows of a (sequence, key head), and shares of the keys so that 512 workgroups (two a CU, all
-// resident) have work, none of them less than 8 groups of 64 tokens.  One token of 64 sequences of up to 4096 (8 key heads, 128
-// features): 61 us with 256 or 512, 65 with 768, 79 with 1024 workgroups; of one sequence of 131071: 40, 42, 47 and 46 us.
+// How a call is cut.  Tiles of 16 rows of a (sequence, key head), or of 128 where these are enough to fill the chip: the
+// large tiles take four times the queries through a CU (8000 keys, 4 x 1024 queries of 32 heads: 242 us against 1063), but a chip
+// has room for 512 of them.  Measured with 8 key heads and 128 features: 512 queries, 128 large tiles, 27 us either way; 100
+// queries, 32 tiles, 18 us with large ones against 11; 16 x 200 queries of 12 heads, 384 tiles, 19 against 23.  float32 takes three
+// products: 4 x 512 queries of 16 heads 106 us with large tiles against 80, 2 x 2000 of 32 heads 260 against 316.
+// Then shares of the keys so that 512 workgroups (two a CU, all resident) have work, none of them less than 8 groups of 64 tokens (16
+// for large tiles).  One token of 64 sequences of up to 4096 (8 key heads, 128 features): 61 us with 256 or 512, 70 with 768 and
+// 68 with 1024 workgroups; of one sequence of 131071: 40, 42, 44 and 45 us.
 struct KvPlan {
-    int tile_rows, tiles, splits;
-    int64_t slots;
+    int tile_rows, tiles, splits;    // tiles of a sequence of `most` rows
+    int64_t slots, grid;
 };
-static KvPlan kv_plan(int sequences, int most, int64_t longest, int heads, int group, int dim, int dtype) {
+static KvPlan kv_plan(int64_t all_rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window, int sinks,
+                      int dtype) {
     KvPlan p;
     const int64_t rows = (int64_t)most * group;
-    p.tile_rows = kv_tile_rows(rows, dim, dtype);
-    p.tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
-    const int64_t base = (int64_t)sequences * heads * p.tiles;
-    p.slots = base * p.tile_rows;
+    if (window > 0 && (int64_t)window + sinks + most < longest) longest = (int64_t)window + sinks + most;     // keys that a tile can see
     const int64_t groups = (longest + kKvGroup - 1) / kKvGroup;
+    int64_t tiles;
+    auto cut = [&](int tile_rows) {
+        p.tile_rows = tile_rows;
+        p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
+        tiles = (int64_t)sequences * p.tiles;
+        p.slots = tiles * heads * tile_rows;
+        // packed rows bound the tiles of all sequences together: whole ones, and one for what is left of each
+        if (tile_rows > 16 && all_rows * group / tile_rows + sequences < tiles) tiles = all_rows * group / tile_rows + sequences;
+    };
+    cut(kKvTileRows);
+    const int64_t large = tiles * heads * (groups < 32 ? 1 : groups / 16);
+    if (rows <= 64 || (dtype == VAMD_F32 ? dim > 128 || large <= 512 : large <= 128)) cut(16);
+    const int64_t base = tiles * heads;
+    const int least = kv_min_share(p.tile_rows);
     int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
-    if (splits > (groups + kKvMinShare - 1) / kKvMinShare) splits = (groups + kKvMinShare - 1) / kKvMinShare;
+    if (splits > (groups + least - 1) / least) splits = (groups + least - 1) / least;
     p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
+    p.grid = base * p.splits;
     return p;
 }
 
@@ -799,7 +885,7 @@ template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, 
 
 template <typename T, int FMT, int DT> static int kv_launch_tile_of(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
     constexpr int LDS = 2 * 2 * DT * 4 * 64 * 16;
-    auto kernel = kv_attend_tile_kernel<T, FMT, DT, CBV>;
+    auto kernel = kv_attend_tile_kernel<T, FMT, DT, 1>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return fail((int)e, "vamd_kv_attend: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
@@ -841,9 +927,10 @@ template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream
 
 using namespace vamd;
 
-extern "C" size_t vamd_kv_attend_workspace(int sequences, int most, int64_t longest, int heads, int group, int dim, int dtype) {
-    if (sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
-    const KvPlan p = kv_plan(sequences, most, longest, heads, group, dim, dtype);
+extern "C" size_t vamd_kv_attend_workspace(int64_t rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window, int sinks,
+                                           int dtype) {
+    if (rows <= 0 || sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
+    const KvPlan p = kv_plan(rows, sequences, most, longest, heads, group, dim, window, sinks, dtype);
     return p.splits > 1 ? (size_t)p.slots * p.splits * (dim + 2) * sizeof(float) : 0;
 }
 
@@ -872,11 +959,11 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE((uintptr_t)codes_k % 16 == 0 && (uintptr_t)codes_v % 16 == 0 && (uintptr_t)scales_k % 4 == 0 && (uintptr_t)scales_v % 4 == 0 &&
                  (uintptr_t)table % 4 == 0 && (uintptr_t)lengths % 4 == 0 && (uintptr_t)offsets % 4 == 0 && (uintptr_t)q % size == 0 &&
                  (uintptr_t)o % size == 0, "vamd_kv_attend: misaligned tensor");
-    const KvPlan plan = kv_plan(sequences, most, longest, heads, group, dim, dtype);
-    const size_t need = vamd_kv_attend_workspace(sequences, most, longest, heads, group, dim, dtype);
+    const KvPlan plan = kv_plan(rows, sequences, most, longest, heads, group, dim, window, sinks, dtype);
+    const size_t need = vamd_kv_attend_workspace(rows, sequences, most, longest, heads, group, dim, window, sinks, dtype);
     VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                  "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    const int64_t grid = plan.slots / plan.tile_rows * plan.splits;
+    const int64_t grid = plan.grid;
     VAMD_REQUIRE(grid <= 0x7fffffff && plan.slots <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
                  sequences, most);
     KvAttendArgs a = {};

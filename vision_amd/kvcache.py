@@ -45,6 +45,7 @@ class KVCache:
         self.scales_k = torch.zeros(shape[:2], dtype=torch.float32, device=device)
         self.scales_v = torch.zeros(shape[:2], dtype=torch.float32, device=device)
         self.device = self.codes_k.device
+        self._index = self.codes_k.get_device()                  # -1 on the CPU
         self._pointers = tuple(t.data_ptr() for t in (self.codes_k, self.codes_v, self.scales_k, self.scales_v))
         self._format = _FORMATS[format]
 
@@ -53,38 +54,48 @@ class KVCache:
     def _rows(self, name, t, heads):
         if t.dtype not in _TYPES:
             raise TypeError(f"{name} is {t.dtype}: float32 or bfloat16")
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, not [rows, {heads}, {self.head_dim}]")
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name} has shape {tuple(shape)}, not [rows, {heads}, {self.head_dim}]")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: the cache passes none (use torch.no_grad())")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         return t if t.stride(2) == 1 else t.contiguous()
 
+    def _numbers(self, name, t, size):
+        """An int32 [size] on the cache's device."""
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not contiguous int32 [{size}]")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+        return t.data_ptr()
+
     def _batch(self, table, what, positions, offsets, rows, most):
-        """Checks the batch's description; returns (sequences, width, rows of a sequence at most)."""
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or table.stride(1) != 1:
-            raise ValueError(f"table: {table.dtype} {tuple(table.shape)}, not int32 [sequences, blocks] with adjacent blocks")
-        n = table.shape[0]
-        for name, t, size in ((what, positions, n), ("offsets", offsets, n + 1)):
-            if t is not None and (t.dtype != torch.int32 or t.shape != (size,) or not t.is_contiguous()):
-                raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, not contiguous int32 [{size}]")
+        """Checks the batch's description; returns the entry points' arguments (table, its stride, positions, offsets), then
+        (sequences, width, rows of a sequence at most)."""
+        shape = table.shape
+        if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or table.stride(1) != 1:
+            raise ValueError(f"table: {table.dtype} {tuple(shape)}, not int32 [sequences, blocks] with adjacent blocks")
+        n, width = shape
+        at = self._numbers(what, positions, n)
         if offsets is None:
             if rows % n:
                 raise ValueError(f"{rows} rows for {n} sequences, and no offsets")
-            if most is not None and most != rows // n:
-                raise ValueError(f"most {most}, but {rows // n} rows each without offsets")
-            most = rows // n
+            each = rows // n
+            if most is not None and most != each:
+                raise ValueError(f"most {most}, but {each} rows each without offsets")
+            most, first = each, None
         else:
+            first = self._numbers("offsets", offsets, n + 1)
             most = rows if most is None else min(int(most), rows)
             if most < 0:
                 raise ValueError(f"most {most}")
-        for name, t in (("table", table), (what, positions), ("offsets", offsets)):
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        if self.device.type != "cuda":
+        if table.get_device() != self._index:
+            raise ValueError(f"table is on {table.device}, the cache on {self.device}")
+        if self._index < 0:
             raise RuntimeError("KVCache runs on the GPU only (libvision_amd.so has no CPU path)")
-        return n, table.shape[1], most
+        return (table.data_ptr(), table.stride(0), at, first), n, width, most
 
     # ---- the operators
 
@@ -97,11 +108,10 @@ class KVCache:
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError(f"k and v differ: {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
         rows = k.shape[0]
-        n, width, most = self._batch(table, "start", start, offsets, rows, most)
+        batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
-        call_on(self.device, "vamd_kv_append", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], *self._pointers, table.data_ptr(),
-                table.stride(0), start.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, n, most, self.kv_heads,
-                self.head_dim, self.block, width, self.blocks, self._format, _TYPES[k.dtype])
+        call_on(self.device, "vamd_kv_append", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], *self._pointers, *batch, rows, n, most,
+                self.kv_heads, self.head_dim, self.block, width, self.blocks, self._format, _TYPES[k.dtype])
 
     def read(self, table, start, rows, offsets=None, most=None, dtype=torch.bfloat16, out=None):
         """(k, v): the values at positions start[b], start[b]+1, ... of each sequence, `rows` rows in all, exact in either dtype; zeros
@@ -119,10 +129,9 @@ class KVCache:
                 self._written(name, t, (rows, self.kv_heads, self.head_dim))
             if k.dtype != v.dtype or k.data_ptr() == v.data_ptr() and k.numel():
                 raise ValueError("out: two different tensors of one dtype")
-        n, width, most = self._batch(table, "start", start, offsets, rows, most)
+        batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
-        call_on(self.device, "vamd_kv_read", *self._pointers, table.data_ptr(), table.stride(0), start.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), rows, n, most, self.kv_heads, self.head_dim, self.block, width,
+        call_on(self.device, "vamd_kv_read", *self._pointers, *batch, rows, n, most, self.kv_heads, self.head_dim, self.block, width,
                 self.blocks, self._format, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _TYPES[k.dtype])
         return k, v
 
@@ -144,20 +153,18 @@ class KVCache:
                 raise ValueError(f"out is {out.dtype}, q {q.dtype}")
             self._apart(q, out)
         rows = q.shape[0]
-        n, width, most = self._batch(table, "lengths", lengths, offsets, rows, most)
+        batch, n, width, most = self._batch(table, "lengths", lengths, offsets, rows, most)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         room = width * self.block
         longest = room if longest is None else min(max(int(longest), 0), room)
         group = heads // self.kv_heads
-        size = lib.vamd_kv_attend_workspace(n, most, longest, self.kv_heads, group, self.head_dim, _TYPES[q.dtype])
+        size = lib.vamd_kv_attend_workspace(rows, n, most, longest, self.kv_heads, group, self.head_dim, window, sinks, _TYPES[q.dtype])
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         qs, os = q.stride(), out.stride()
-        call_on(self.device, "vamd_kv_attend", q.data_ptr(), qs[0], qs[1], *self._pointers, table.data_ptr(), table.stride(0),
-                lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, n, most, longest, self.kv_heads, group,
-                self.head_dim, self.block, width, self.blocks, self._format, self.head_dim ** -0.5 if scale is None else float(scale),
-                int(bool(causal)), window, sinks, out.data_ptr(), os[0], os[1], None if work is None else work.data_ptr(), size,
-                _TYPES[q.dtype])
+        call_on(self.device, "vamd_kv_attend", q.data_ptr(), qs[0], qs[1], *self._pointers, *batch, rows, n, most, longest, self.kv_heads,
+                group, self.head_dim, self.block, width, self.blocks, self._format, self.head_dim ** -0.5 if scale is None else float(scale),
+                bool(causal), window, sinks, out.data_ptr(), os[0], os[1], None if work is None else work.data_ptr(), size, _TYPES[q.dtype])
         return out
 
     def _written(self, name, t, shape):

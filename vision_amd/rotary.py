@@ -91,8 +91,9 @@ def _args(t, o, lead):
             raise ValueError(f"a tensor with strides {t.stride()} cannot be turned in place together with the other one")
         t = t.contiguous()
         a = _layout(t, lead)
-    b = a if o is t else _layout(o, a[:2])
-    return t, (t.data_ptr(), o.data_ptr(), t.shape[-2], a[2], a[3], a[4], b[2], b[3], b[4]), a[:2]
+    batch, tokens, x0, x1, x2 = a
+    y0, y1, y2 = (x0, x1, x2) if o is t or o.stride() == t.stride() else _layout(o, (batch, tokens))[2:]
+    return (t.data_ptr(), o.data_ptr(), t.shape[-2], x0, x1, x2, y0, y1, y2), (batch, tokens), t
 
 
 _NONE = (None, None, 0, 0, 0, 0, 0, 0, 0)
@@ -102,11 +103,11 @@ def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, q, k,
     """One launch for up to two tensors of equal leading dimensions; q or k may be None."""
     ref, lead, aq, ak = q, None, _NONE, _NONE
     if q is not None:
-        q, aq, lead = _args(q, yq, None)
+        aq, lead, q = _args(q, yq, None)             # (a copy that had to be made lives until the launch)
     else:
         ref = k
     if k is not None:
-        k, ak, lead = _args(k, yk, lead)
+        ak, lead, k = _args(k, yk, lead)
     if positions.dim() != ref.dim() - 2 or positions.shape != ref.shape[:-2]:
         positions = positions.expand(ref.shape[:-2])
     if not positions.is_contiguous():
@@ -172,27 +173,28 @@ class Rotary(nn.Module):
         self._how = (self.amplitude, rotary_dim, int(layout == "interleaved"), 0)
 
     def _check(self, positions, q, k):
-        for name, t in (("q", q), ("k", k)):
-            if t is None:
-                continue
-            if t.dtype not in _TYPES:
-                raise TypeError(f"{name} is {t.dtype}: float32 or bfloat16")
-            if t.dim() < 2 or t.shape[-1] != self.head_dim:
-                raise ValueError(f"{name} has shape {tuple(t.shape)}, not [..., heads, {self.head_dim}]")
-        if k is not None and (k.dtype != q.dtype or k.shape[:-2] != q.shape[:-2] or k.device != q.device):
-            raise ValueError(f"q and k differ: {q.dtype} {tuple(q.shape)} on {q.device}, {k.dtype} {tuple(k.shape)} on {k.device}")
-        if positions.dtype not in (torch.int32, torch.int64):
+        shape, dtype = q.shape, q.dtype
+        if dtype not in _TYPES:
+            raise TypeError(f"q is {dtype}: float32 or bfloat16")
+        if len(shape) < 2 or shape[-1] != self.head_dim:
+            raise ValueError(f"q has shape {tuple(shape)}, not [..., heads, {self.head_dim}]")
+        lead, index = shape[:-2], q.get_device()
+        if k is not None and (k.dtype != dtype or k.shape[-1] != self.head_dim or k.shape[:-2] != lead or k.get_device() != index):
+            raise ValueError(f"q and k differ: {dtype} {tuple(shape)} on {q.device}, {k.dtype} {tuple(k.shape)} on {k.device}")
+        if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"positions are {positions.dtype}: int32 or int64")
-        lead, have = q.shape[:-2], positions.shape
+        have = positions.shape
         if have != lead and (len(have) > len(lead) or any(n not in (1, m) for n, m in zip(reversed(have), reversed(lead)))):
             raise ValueError(f"positions have shape {tuple(have)}, not {tuple(lead)} or broadcast to it")
         if not q.is_cuda:
             raise RuntimeError("Rotary runs on the GPU only (libvision_amd.so has no CPU path)")
-        if positions.device != q.device or self.frequencies.device != q.device:
-            raise ValueError(f"q is on {q.device}, positions on {positions.device}, the frequencies on {self.frequencies.device}")
+        frequencies = self._buffers["frequencies"]
+        if positions.get_device() != index or frequencies.get_device() != index:
+            raise ValueError(f"q is on {q.device}, positions on {positions.device}, the frequencies on {frequencies.device}")
+        return frequencies
 
     def forward(self, positions, q, k=None):
-        self._check(positions, q, k)
+        frequencies = self._check(positions, q, k)
         if q.numel() == 0 or (k is not None and k.numel() == 0):
             if k is None:
                 return q.clone()
@@ -202,12 +204,12 @@ class Rotary(nn.Module):
         turn = _turned
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             turn = _RotaryFn.apply
-        yq, yk = turn(positions, self.frequencies, self._how, q, k)
+        yq, yk = turn(positions, frequencies, self._how, q, k)
         return yq if k is None else (yq, yk)
 
     def apply_(self, positions, q, k=None):
         """Turns q and k in place and returns them; for inference (no gradient passes through it)."""
-        self._check(positions, q, k)
+        frequencies = self._check(positions, q, k)
         for name, t in (("q", q), ("k", k)):
             if t is None:
                 continue
@@ -224,5 +226,5 @@ class Rotary(nn.Module):
             if k is not None and (q.numel() or k.numel()):
                 self.apply_(positions, q if q.numel() else k)
             return q if k is None else (q, k)
-        _turn(positions, self.frequencies, *self._how, q, k, q, k)
+        _turn(positions, frequencies, *self._how, q, k, q, k)
         return q if k is None else (q, k)
