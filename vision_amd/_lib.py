@@ -162,6 +162,7 @@ SIGNATURES = {
     "vamd_rotary": (_i, [_p, _i, _p, _f, _l, _l, _i, _i, _i, _i] + [_p, _p, _i, _l, _l, _l, _l, _l, _l] * 2 + [_i, _p]),
     "vamd_kv_append": (_i, [_p, _l, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _p, _l] + [_i] * 9 + [_p]),
     "vamd_kv_read": (_i, [_p, _p, _p, _p, _p, _l, _p, _p, _l] + [_i] * 8 + [_p, _l, _l, _p, _l, _l, _i, _p]),
+    "vamd_kv_attend_tile": (_i, [_l, _i, _i, _l, _i, _i, _i, _i, _i, _i]),
     "vamd_kv_attend_workspace": (_z, [_l, _i, _i, _l, _i, _i, _i, _i, _i, _i]),
     "vamd_kv_attend": (_i, [_p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _p, _l, _i, _i, _l] + [_i] * 7 +
                        [_f, _i, _i, _i, _p, _l, _l, _p, _z, _i, _p]),

@@ -861,7 +861,7 @@ static KvPlan kv_plan(int64_t all_rows, int sequences, int most, int64_t longest
     const int64_t base = tiles * heads;
     const int least = kv_min_share(p.tile_rows);
     int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
-    if (splits > (groups + least - 1) / least) splits = (groups + least - 1) / least;
+    if (splits > groups / least) splits = groups / least;
     p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
     p.grid = base * p.splits;
     return p;
@@ -932,6 +932,12 @@ extern "C" size_t vamd_kv_attend_workspace(int64_t rows, int sequences, int most
     if (rows <= 0 || sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
     const KvPlan p = kv_plan(rows, sequences, most, longest, heads, group, dim, window, sinks, dtype);
     return p.splits > 1 ? (size_t)p.slots * p.splits * (dim + 2) * sizeof(float) : 0;
+}
+
+extern "C" int vamd_kv_attend_tile(int64_t rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window, int sinks,
+                                   int dtype) {
+    if (rows <= 0 || sequences <= 0 || most <= 0 || heads <= 0 || group <= 0 || dim <= 0) return 0;
+    return kv_plan(rows, sequences, most, longest, heads, group, dim, window, sinks, dtype).tile_rows;
 }
 
 extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, const void* codes_k, const void* codes_v,

@@ -6,8 +6,9 @@
 //   2. the scale: for a block that the call begins at its first token, what that maximum needs; otherwise the larger of that and
 //      the block's scale.  A scale is a power of two, so moving a block to a larger one is an exact product by old / new in
 //      32 bits and one rounding to the code: e4m3 codes only lose bits that fall below the smallest code, int8 codes round again;
-//   3. the rows again (from the caches), as codes: x * 2^-e is exact, the code's rounding (to nearest, ties to even) is the only one.
-// Bound by memory; the second read of the rows comes from L2.  A block belongs to one sequence while it is written: no two
+//   3. the rows as codes, from registers where a workgroup can hold them, else read again (from L2): x * 2^-e is exact, the code's
+//      rounding (to nearest, ties to even) is the only one.
+// Bound by memory: 16000 tokens of 8 heads and 128 features (int8, blocks of 128) 28 us written, 21 read back, 3.6 and 4.8 TB/s.  A block belongs to one sequence while it is written: no two
 // workgroups of a call write the same bytes, nothing is added atomically, the result does not depend on any order.
 #include "kv_layout.h"
 
@@ -27,6 +28,13 @@ struct KvIoArgs {
     int heads, D, block, width, blocks, most, touched;
 };
 
+template <typename T, bool ALIGNED> __device__ __forceinline__ Vec16<T> kv_load16(const T* p) {
+    if (ALIGNED) return *(const Vec16<T>*)p;
+    Vec16<T> w;
+#pragma unroll
+    for (int e = 0; e < Vec16<T>::N; ++e) w.v[e] = p[e];
+    return w;
+}
 template <typename T, bool ALIGNED> __device__ __forceinline__ void kv_load8(const T* p, float (&v)[8]) {
     if (ALIGNED) {
 #pragma unroll
@@ -60,7 +68,7 @@ template <int FMT> __device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, f
     return kv_encode4<FMT>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
 }
 
-template <typename T, int FMT, bool ALIGNED>
+template <typename T, int FMT, bool ALIGNED, int HOLD>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     __shared__ uint32_t tops[4];
     int64_t id = blockIdx.x;
@@ -78,18 +86,77 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     const int page = kv_page(a.table, a.table_stride, a.width, a.blocks, b, blk);
     if (page < 0) return;
 
-    const int tid = threadIdx.x, nt = blockDim.x, D = a.D, P = D >> 3;
+    const int tid = threadIdx.x, nt = blockDim.x, D = a.D, P = D >> 3, S = D >> 4;
     const int64_t tok = a.tok[kv];
     const T* x = (const T*)a.x[kv] + (rows.first + base - start) * tok + h * a.head[kv];     // row of token 0 of the block
+    // What a lane quantises later it keeps in registers where that is little (HOLD times 32 elements): pieces of keys are 16
+    // features of a token, of values 8 features of 4 neighbouring tokens; `pieces` and `quads` of them in a group of 64 tokens.
+    const int pieces = kKvGroup * S, quads = 16 * P;
+    const int f0 = lo / kKvGroup, f1 = (hi + kKvGroup - 1) / kKvGroup;          // groups with fresh tokens
+    const int items = (f1 - f0) * (kv == 0 ? pieces : quads), per = kv == 0 ? 2 * HOLD : HOLD;
+    const bool held = items <= per * nt;
+    auto key_place = [&](int i, int& g, int& q, int& t, int& d) {
+        g = i / pieces;
+        q = i - g * pieces;
+        t = g * kKvGroup + (q >> 4) / S * 16 + (q & 15);
+        d = (q >> 4) % S * 16;
+    };
+    auto value_place = [&](int i, int& g, int& t, int& p, int& gg, int& tt) {
+        g = i / quads;
+        const int q = i - g * quads;
+        tt = q & 3;
+        p = (q >> 2) % P;
+        gg = (q >> 2) / P;
+        t = g * kKvGroup + tt * 16 + gg * 4;
+    };
+    Vec16<T> kept[HOLD][32 * sizeof(T) / 16];
     uint32_t top = 0;
-    for (int i = tid; i < (hi - lo) * P; i += nt) {
-        const int t = lo + i / P, p = i % P;
-        float v[8];
-        kv_load8<T, ALIGNED>(x + t * tok + p * 8, v);
+    auto look = [&](const Vec16<T>& w) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+        for (int e = 0; e < Vec16<T>::N; ++e) {
+            const uint32_t m = __float_as_uint(to_f(w.v[e])) & 0x7fffffffu;
             top = m > top ? m : top;
+        }
+    };
+    constexpr int V8 = 8 / Vec16<T>::N;                          // 16-byte vectors of 8 elements
+    if (held && kv == 0) {
+#pragma unroll
+        for (int n = 0; n < 2 * HOLD; ++n) {
+            int g, q, t = hi, d = 0;
+            const int i = tid + n * nt;
+            if (i < items) key_place(i + f0 * pieces, g, q, t, d);
+#pragma unroll
+            for (int e = 0; e < 2 * V8; ++e) {
+                Vec16<T> w = {};
+                if (t >= lo && t < hi) w = kv_load16<T, ALIGNED>(x + t * tok + d + e * Vec16<T>::N);
+                kept[n >> 1][(n & 1) * 2 * V8 + e] = w;
+            }
+        }
+    } else if (held) {
+#pragma unroll
+        for (int n = 0; n < HOLD; ++n) {
+            int g, t = hi, p = 0, gg, tt;
+            const int i = tid + n * nt;
+            if (i < items) value_place(i + f0 * quads, g, t, p, gg, tt);
+#pragma unroll
+            for (int e = 0; e < 4 * V8; ++e) {
+                Vec16<T> w = {};
+                const int tn = t + e / V8;
+                if (tn >= lo && tn < hi) w = kv_load16<T, ALIGNED>(x + tn * tok + p * 8 + e % V8 * Vec16<T>::N);
+                kept[n][e] = w;
+            }
+        }
+    }
+    if (held) {
+#pragma unroll
+        for (int n = 0; n < HOLD; ++n)
+#pragma unroll
+            for (int e = 0; e < 4 * V8; ++e) look(kept[n][e]);
+    } else {
+        for (int i = tid; i < (hi - lo) * P; i += nt) {
+            const int t = lo + i / P, p = i % P;
+#pragma unroll
+            for (int e = 0; e < V8; ++e) look(kv_load16<T, ALIGNED>(x + t * tok + p * 8 + e * Vec16<T>::N));
         }
     }
 #pragma unroll
@@ -118,50 +185,105 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     if (tid == 0 && now != old) *scale = __uint_as_float(now);
 
     uint8_t* codes = a.codes[kv] + ((int64_t)page * a.heads + h) * a.block * D;
-    const int g0 = grow ? 0 : lo / kKvGroup, g1 = grow ? a.block / kKvGroup : (hi + kKvGroup - 1) / kKvGroup;
-    if (kv == 0) {
-        const int S = D >> 4, pieces = kKvGroup * S;             // 16-byte pieces of a group: 16 features of one token
-        for (int i = tid; i < (g1 - g0) * pieces; i += nt) {
-            const int g = g0 + i / pieces, q = i % pieces;
-            const int t = g * kKvGroup + (q >> 4) / S * 16 + (q & 15), d = (q >> 4) % S * 16;
-            const bool fresh = t >= lo && t < hi;
-            if (!fresh && !grow) continue;
-            kv_u32x4* to = (kv_u32x4*)(codes + (int64_t)g * kKvGroup * D) + q;
-            kv_u32x4 w;
-            if (fresh) {
+    auto encode_key = [&](const float (&v)[16]) {
+        kv_u32x4 w;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v[8];
-                    kv_load8<T, ALIGNED>(x + t * tok + d + e * 8, v);
-                    w[2 * e] = dead ? 0u : kv_encode4<FMT>(fit(v[0]), fit(v[1]), fit(v[2]), fit(v[3]));
-                    w[2 * e + 1] = dead ? 0u : kv_encode4<FMT>(fit(v[4]), fit(v[5]), fit(v[6]), fit(v[7]));
-                }
-            } else {
-                w = *to;
+        for (int e = 0; e < 4; ++e)
+            w[e] = dead ? 0u : kv_encode4<FMT>(fit(v[4 * e]), fit(v[4 * e + 1]), fit(v[4 * e + 2]), fit(v[4 * e + 3]));
+        return w;
+    };
+    // codes of four tokens of one feature, from the features' rows
+    auto encode_quad = [&](const float (&v)[4][8], int e) {
+        return dead ? 0u : kv_encode4<FMT>(fit(v[0][e]), fit(v[1][e]), fit(v[2][e]), fit(v[3][e]));
+    };
+    auto quad_at = [&](int g, int p, int gg, int tt) {
+        return codes + (int64_t)g * kKvGroup * D + (((p >> 1) * 4 + gg) * 16 + (p & 1) * 8) * 16 + tt * 4;
+    };
+    // stores the fresh tokens of a quad (t ..): whole dwords, or their bytes beside others that stay
+    auto put_quad = [&](uint8_t* to, const float (&v)[4][8], int t) {
+        const bool all = t >= lo && t + 4 <= hi;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t c = encode_quad(v, e);
+            if (all) *(uint32_t*)(to + e * 16) = c;
+            else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (t + n >= lo && t + n < hi) to[e * 16 + n] = (uint8_t)(c >> (8 * n));
+            }
+        }
+    };
+    if (grow) {
+        // every other code of the block moves to the new scale (what is fresh is written behind this, by the lanes below)
+        const int groups = a.block / kKvGroup;
+        if (kv == 0) {
+            for (int i = tid; i < groups * pieces; i += nt) {
+                int g, q, t, d;
+                key_place(i, g, q, t, d);
+                if (t >= lo && t < hi) continue;
+                kv_u32x4* to = (kv_u32x4*)(codes + (int64_t)g * kKvGroup * D) + q;
+                kv_u32x4 w = *to;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = old ? kv_rescale4<FMT>(w[e], ratio) : 0u;
+                *to = w;
             }
-            *to = w;
+        } else {
+            for (int i = tid; i < groups * quads; i += nt) {
+                int g, t, p, gg, tt;
+                value_place(i, g, t, p, gg, tt);
+                if (t >= lo && t + 4 <= hi) continue;
+                uint8_t* to = quad_at(g, p, gg, tt);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) *(uint32_t*)(to + e * 16) = old ? kv_rescale4<FMT>(*(const uint32_t*)(to + e * 16), ratio) : 0u;
+            }
+            __syncthreads();                                     // fresh bytes go into these dwords
+        }
+    }
+    if (kv == 0) {
+        auto put = [&](int i, const float (&v)[16]) {
+            int g, q, t, d;
+            key_place(i + f0 * pieces, g, q, t, d);
+            if (t >= lo && t < hi) *((kv_u32x4*)(codes + (int64_t)g * kKvGroup * D) + q) = encode_key(v);
+        };
+        if (held) {
+#pragma unroll
+            for (int n = 0; n < 2 * HOLD; ++n) {
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = to_f(kept[n >> 1][(n & 1) * 2 * V8 + e / Vec16<T>::N].v[e % Vec16<T>::N]);
+                if (tid + n * nt < items) put(tid + n * nt, v);
+            }
+        } else {
+            for (int i = tid; i < items; i += nt) {
+                int g, q, t, d;
+                key_place(i + f0 * pieces, g, q, t, d);
+                if (t < lo || t >= hi) continue;
+                float v[16], u[2][8];
+                kv_load8<T, ALIGNED>(x + t * tok + d, u[0]);
+                kv_load8<T, ALIGNED>(x + t * tok + d + 8, u[1]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = u[e >> 3][e & 7];
+                put(i, v);
+            }
         }
     } else {
-        // dwords of a group: four neighbouring tokens of one feature; a lane makes those of eight features
-        const int quads = 16 * P;
-        for (int i = tid; i < (g1 - g0) * quads; i += nt) {
-            const int g = g0 + i / quads, q = i % quads;
-            const int tt = q & 3, p = (q >> 2) % P, gg = (q >> 2) / P;
-            const int t = g * kKvGroup + tt * 16 + gg * 4;
-            const bool any = t < hi && t + 4 > lo, all = t >= lo && t + 4 <= hi;
-            if (!any && !grow) continue;
-            uint8_t* to = codes + (int64_t)g * kKvGroup * D + (((p >> 1) * 4 + gg) * 16 + (p & 1) * 8) * 16 + tt * 4;
-            uint32_t w[8] = {};
-            if (!all && !(grow && !old)) {
+        if (held) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = *(const uint32_t*)(to + e * 16);
-                    if (grow) w[e] = kv_rescale4<FMT>(w[e], ratio);
+            for (int n = 0; n < HOLD; ++n) {
+                float v[4][8];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e >> 3][e & 7] = to_f(kept[n][e / Vec16<T>::N].v[e % Vec16<T>::N]);
+                int g, t, p, gg, tt;
+                if (tid + n * nt < items) {
+                    value_place(tid + n * nt + f0 * quads, g, t, p, gg, tt);
+                    if (t < hi && t + 4 > lo) put_quad(quad_at(g, p, gg, tt), v, t);
                 }
             }
-            if (any) {
+        } else {
+            for (int i = tid; i < items; i += nt) {
+                int g, t, p, gg, tt;
+                value_place(i + f0 * quads, g, t, p, gg, tt);
+                if (t >= hi || t + 4 <= lo) continue;
                 float v[4][8];
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
@@ -171,17 +293,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
                         for (int e = 0; e < 8; ++e) v[n][e] = 0.f;
                     }
                 }
-                uint32_t keep = 0;                               // bytes of tokens that this call does not write
-#pragma unroll
-                for (int n = 0; n < 4; ++n) keep |= t + n >= lo && t + n < hi ? 0u : 255u << (8 * n);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t c = dead ? 0u : kv_encode4<FMT>(fit(v[0][e]), fit(v[1][e]), fit(v[2][e]), fit(v[3][e]));
-                    w[e] = (w[e] & keep) | (c & ~keep);
-                }
+                put_quad(quad_at(g, p, gg, tt), v, t);
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) *(uint32_t*)(to + e * 16) = w[e];
         }
     }
 }
@@ -281,15 +394,20 @@ static bool kv_aligned(const KvIoArgs& a, const void* p, const void* q, int dtyp
     return (uintptr_t)p % 16 == 0 && (uintptr_t)q % 16 == 0 && a.tok[0] % n == 0 && a.tok[1] % n == 0 && a.head[0] % n == 0 && a.head[1] % n == 0;
 }
 
-#define KV_IO_LAUNCH(kernel, T, aligned)                                                                             \
-    do {                                                                                                             \
-        if (format == VAMD_KV_E4M3) {                                                                                \
-            if (aligned) hipLaunchKernelGGL((kernel<T, VAMD_KV_E4M3, true>), dim3((unsigned)grid), dim3(threads), 0, as_stream(stream), a);   \
-            else hipLaunchKernelGGL((kernel<T, VAMD_KV_E4M3, false>), dim3((unsigned)grid), dim3(threads), 0, as_stream(stream), a);          \
-        } else {                                                                                                     \
-            if (aligned) hipLaunchKernelGGL((kernel<T, VAMD_KV_INT8, true>), dim3((unsigned)grid), dim3(threads), 0, as_stream(stream), a);   \
-            else hipLaunchKernelGGL((kernel<T, VAMD_KV_INT8, false>), dim3((unsigned)grid), dim3(threads), 0, as_stream(stream), a);          \
-        }                                                                                                            \
+#define COMMA ,
+// KERNEL, which names T, F (format) and A (aligned), for this call's format and alignment; T from VAMD_DISPATCH around it
+#define KV_IO_LAUNCH(KERNEL)                                                                                                     \
+    do {                                                                                                                         \
+        const dim3 g((unsigned)grid), t(threads);                                                                                \
+        if (format == VAMD_KV_E4M3) {                                                                                            \
+            constexpr int F = VAMD_KV_E4M3;                                                                                      \
+            if (aligned) { constexpr bool A = true; hipLaunchKernelGGL((KERNEL), g, t, 0, as_stream(stream), a); }                \
+            else { constexpr bool A = false; hipLaunchKernelGGL((KERNEL), g, t, 0, as_stream(stream), a); }                       \
+        } else {                                                                                                                 \
+            constexpr int F = VAMD_KV_INT8;                                                                                      \
+            if (aligned) { constexpr bool A = true; hipLaunchKernelGGL((KERNEL), g, t, 0, as_stream(stream), a); }                \
+            else { constexpr bool A = false; hipLaunchKernelGGL((KERNEL), g, t, 0, as_stream(stream), a); }                       \
+        }                                                                                                                        \
     } while (0)
 
 }  // namespace vamd
@@ -317,7 +435,11 @@ extern "C" int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, co
     const bool aligned = kv_aligned(a, k, v, dtype);
     // One wave where a block gets at most 4 tokens (a decoding step: no barrier, more blocks a CU), else four.
     const int threads = most <= 4 ? 64 : 256;
-    VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel, T, aligned););
+    // What four waves hold in registers: blocks up to 16384 elements (64 or 128 tokens of 128 features) with HOLD 2, up to 32768 with 4
+    // (116 and 180 registers; beyond that the rows are read twice).  16000 tokens of 8 heads, 128 features, written and read back: blocks of
+    // 128 tokens 55 us with 2, 66 with 4, 67 read twice; of 256 tokens 60 with 4, 71 read twice.
+    if (block * dim <= 16384 || threads == 64) VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 2>););
+    else VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 4>););
     VAMD_LAUNCH_OK("kv_append");
     return 0;
 }
@@ -342,7 +464,7 @@ extern "C" int vamd_kv_read(const void* codes_k, const void* codes_v, const floa
     a.head[1] = v_head;
     const bool aligned = kv_aligned(a, k, v, dtype);
     const int threads = 256;
-    VAMD_DISPATCH(dtype, "vamd_kv_read", KV_IO_LAUNCH(kv_read_kernel, T, aligned););
+    VAMD_DISPATCH(dtype, "vamd_kv_read", KV_IO_LAUNCH(kv_read_kernel<T COMMA F COMMA A>););
     VAMD_LAUNCH_OK("kv_read");
     return 0;
 }
