@@ -347,7 +347,7 @@ def test_large_tiles_values_of_any_scale():
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
 def test_large_tiles_split_and_joined(dtype):
-    H, G, D = (8, 2, 64) if dtype == torch.bfloat16 else (16, 2, 64)
+    H, G, D = (8, 2, 64) if dtype == torch.bfloat16 else (20, 2, 64)
     lengths, counts = [6100, 3000, 40, 1500, 5000, 700], [40, 64, 40, 1, 33, 0]
     c, table, k, v, off = filled(lengths, H, D, 64, "int8", 280)
     q = rnd((sum(counts), H * G, D), dtype, 289)
@@ -397,6 +397,24 @@ def test_many_sequences():
     c, table, k, v, off = filled(lengths, H, D, 64, "e4m3", 320)
     q = rnd((sum(counts), H, D), torch.bfloat16, 329)
     compare(attend_large(c, q, table, lengths, counts, H, 1, D, torch.bfloat16), q, k, v, off, lengths, counts, D ** -0.5, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
+@pytest.mark.parametrize("sequences,H", [(3, 2), (50, 16)])
+def test_rows_beyond_most_are_left_out(dtype, sequences, H):
+    """... and the others keep their positions; small and large tiles."""
+    lengths, counts, most = [200] * sequences, [90 - i % 3 * 40 for i in range(sequences)], 70
+    c, table, k, v, off = filled(lengths, H, 32, 64, "e4m3", 340)
+    o = offsets_of(counts)
+    q = rnd((o[-1], H, 32), dtype, 349)
+    t = _lib.F32 if dtype == torch.float32 else _lib.BF16
+    assert lib.vamd_kv_attend_tile(o[-1], sequences, most, 200, H, 1, 32, 0, 0, t) == (16 if sequences == 3 else 128)
+    want = c.attend(q, table, i32(lengths), offsets=i32(o), most=max(counts), longest=200)
+    got = c.attend(q, table, i32(lengths), offsets=i32(o), most=most, longest=200, out=torch.full_like(q, 7.0))
+    compare(want, q, k, v, off, lengths, counts, 32 ** -0.5, dtype)
+    for b, n in enumerate(counts):
+        assert torch.allclose(got[o[b]:o[b] + min(n, most)].float(), want[o[b]:o[b] + min(n, most)].float(), atol=2e-2, rtol=2e-2)
+        assert (got[o[b] + min(n, most):o[b + 1]] == 7).all()
 
 
 def test_no_rows():

@@ -155,6 +155,7 @@ def _i32(*n):
     ("read", ValueError, lambda: dict(out=(torch.zeros(2, 2, 32), torch.zeros(2, 2, 32).bfloat16()))),
     ("read", ValueError, lambda: dict(out=(torch.zeros(2, 2, 32), torch.zeros(1, 2, 32).expand(2, 2, 32)))),
     ("read", ValueError, lambda: dict(out=(torch.zeros(2, 2, 32),) * 2)),
+    ("read", ValueError, lambda: (lambda x: dict(out=(x[:2], x[1:])))(torch.zeros(3, 2, 32))),
     ("read", ValueError, lambda: dict(out=(torch.zeros(2, 2, 64)[..., ::2], torch.zeros(2, 2, 32)))),
     ("attend", ValueError, lambda: dict(q=torch.zeros(2, 5, 32))),
     ("attend", ValueError, lambda: dict(q=torch.zeros(2, 0, 32))),
@@ -176,7 +177,7 @@ def test_cache_call_refuses(method, error, bad):
 
 def test_attend_refuses_overlapping_out():
     x = torch.zeros(3, 6, 32)
-    with pytest.raises(ValueError, match="shares memory"):
+    with pytest.raises(ValueError, match="share memory"):
         _call("attend", q=x[:2], out=x[1:])
 
 
@@ -253,7 +254,7 @@ int main(int argc, char** argv) {
     const int32_t off[6] = {-5, 3, 2, 100, 2147483647, 7};
     for (int b = 0; b < 5; ++b) for (int most = 0; most < 12; ++most) {
         const KvRows r = kv_rows(off, b, 10, most);
-        if (r.first < 0 || r.count < 0 || r.count > most || r.first + r.count > 10) return 5;
+        if (r.first < 0 || r.count < 0 || r.count > most || r.first + r.count > 10 || r.all < r.count || r.first + r.all > 10) return 5;
     }
     if (kv_rows(NULL, 3, 20, 5).first != 15 || kv_rows(NULL, 3, 20, 5).count != 5) return 6;
     // every row of a call falls into one span; a negative start into none

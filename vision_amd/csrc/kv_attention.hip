@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     if (tile * 16 >= rows.count * a.group) return;
     const int length = kv_length(a, b);
-    const int shift = length - rows.count;                               // position of the sequence's first query
+    const int shift = length - (int)rows.all;                               // position of the sequence's first query
     const int row = tile * 16 + r, tok = row / a.group;
     const bool live = tok < rows.count;
     const int pos = a.causal ? shift + tok : length - 1;
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
     if (tile < 0) return;
     const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * a.tile_rows;
     const int first_row = tile * a.tile_rows;
-    const int length = kv_length(a, b), shift = length - rows.count;
+    const int length = kv_length(a, b), shift = length - (int)rows.all;
     const int last_row = first_row + a.tile_rows - 1 < all_rows ? first_row + a.tile_rows - 1 : all_rows - 1;
     const int p_first = a.causal ? shift + first_row / a.group : length - 1, p_last = a.causal ? shift + last_row / a.group : length - 1;
     const KvRange range = kv_range(a, length, p_first, p_last);
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int tok = row / a.group;
     if (tok >= rows.count) return;
-    const int length = kv_length(a, b), shift = length - rows.count, r0 = row / a.tile_rows * a.tile_rows;
+    const int length = kv_length(a, b), shift = length - (int)rows.all, r0 = row / a.tile_rows * a.tile_rows;
     const int r1 = r0 + a.tile_rows < rows.count * a.group ? r0 + a.tile_rows - 1 : rows.count * a.group - 1;
     const KvRange range = kv_range(a, length, a.causal ? shift + r0 / a.group : length - 1, a.causal ? shift + r1 / a.group : length - 1);
     const int per = kv_share(range.count, a.splits, a.tile_rows);
@@ -956,7 +956,8 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE(window >= 0 && sinks >= 0 && (causal || window == 0), "vamd_kv_attend: window %d, sinks %d (not negative; a window "
                  "needs causal queries)", window, sinks);
     VAMD_REQUIRE((int64_t)width * block <= 0x7fffffc0, "vamd_kv_attend: %d blocks of %d tokens are too many for a sequence", width, block);
-    VAMD_REQUIRE((int64_t)most * group <= 0x7fffffc0, "vamd_kv_attend: %d rows of %d heads are too many for a sequence", most, group);
+    VAMD_REQUIRE((int64_t)most * group <= 0x7fffffc0 && rows <= 0x7fffffff, "vamd_kv_attend: %d of %lld rows of %d heads are too many for a sequence",
+                 most, (long long)rows, group);
     VAMD_REQUIRE(offsets || rows == (int64_t)sequences * most, "vamd_kv_attend: %lld rows are not %d for each of %d sequences",
                  (long long)rows, most, sequences);
     if (rows == 0 || most == 0) return 0;
@@ -970,7 +971,7 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                  "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     const int64_t grid = plan.grid;
-    VAMD_REQUIRE(grid <= 0x7fffffff && plan.slots <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
+    VAMD_REQUIRE(grid <= 0x7fffffff && (plan.splits == 1 || plan.slots <= 0x7fffffff), "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
                  sequences, most);
     KvAttendArgs a = {};
     a.q = q;

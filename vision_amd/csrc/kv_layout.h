@@ -79,17 +79,19 @@ template <int FMT> __host__ __device__ __forceinline__ uint32_t kv_scale_bits(ui
 // ---- where a call's rows and blocks are; nothing that a table, a start or an offset holds leads outside the tensors.
 // (host code too: tests run these on the CPU)
 
-// Rows of sequence b in a packed batch of `rows`: first .. first + count - 1.  offsets == NULL: every sequence has `most` rows.
+// Rows of sequence b in a packed batch of `rows`: first .. first + count - 1, of `all` that the sequence has (the others lie beyond
+// `most` and are left out).  offsets == NULL: every sequence has `most` rows.
 struct KvRows {
     int64_t first;
     int count;
+    int64_t all;
 };
 __host__ __device__ __forceinline__ KvRows kv_rows(const int32_t* offsets, int b, int64_t rows, int most) {
-    if (!offsets) return KvRows{(int64_t)b * most, most};
+    if (!offsets) return KvRows{(int64_t)b * most, most, most};
     int64_t lo = offsets[b], hi = offsets[b + 1];
     lo = lo < 0 ? 0 : lo > rows ? rows : lo;
     hi = hi < lo ? lo : hi > rows ? rows : hi;
-    return KvRows{lo, (int)(hi - lo < most ? hi - lo : most)};
+    return KvRows{lo, (int)(hi - lo < most ? hi - lo : most), hi - lo};
 }
 // Tokens lo .. hi - 1 of the unit (block or group) that starts at position `base`, for rows at start .. start + count - 1.
 struct KvSpan {

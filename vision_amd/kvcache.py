@@ -13,9 +13,11 @@ each sequence in order, entries outside 0 .. blocks-1 are holes.  Each (block, h
 for its values; a block's scale starts with the write of its first token and never shrinks after that.
 Rows k, v [rows, kv_heads, head_dim], q and out [rows, heads, head_dim] (heads a multiple of kv_heads; head h reads key head
 h // (heads // kv_heads)) are float32 or bfloat16 with any strides and adjacent features; packed one sequence after the other:
-sequence b owns rows offsets[b] .. offsets[b+1]-1 (`offsets` int32, [sequences + 1]; `most`: a bound of their number, the rows beyond it are
-left out), or without `offsets` rows / sequences each.  `start`, `lengths`: int32, [sequences], on the GPU; nothing
-is copied to the host, so all of it can be captured into a graph.  Rows behind the last sequence are neither read nor written.
+sequence b owns rows offsets[b] .. offsets[b+1]-1 (`offsets` int32, [sequences + 1]), or without `offsets` rows / sequences each.
+`most` bounds the rows of a sequence where the caller knows it: launches are sized by it (default: all rows), rows of a sequence beyond
+it are left out.  `start`, `lengths`: int32, [sequences], on the GPU; nothing
+is copied to the host, so all of it can be captured into a graph.  Rows behind the last sequence are neither read nor written (in a
+result that the call allocates they hold nothing in particular).
 
 The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no gradient.
 """
@@ -127,8 +129,9 @@ class KVCache:
             k, v = out
             for name, t in (("out[0]", k), ("out[1]", v)):
                 self._written(name, t, (rows, self.kv_heads, self.head_dim))
-            if k.dtype != v.dtype or k.data_ptr() == v.data_ptr() and k.numel():
-                raise ValueError("out: two different tensors of one dtype")
+            if k.dtype != v.dtype:
+                raise ValueError(f"out: {k.dtype} and {v.dtype}")
+            self._apart("out's two tensors", k, v)
         batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
         call_on(self.device, "vamd_kv_read", *self._pointers, *batch, rows, n, most, self.kv_heads, self.head_dim, self.block, width,
@@ -151,7 +154,9 @@ class KVCache:
             self._written("out", out, q.shape)
             if out.dtype != q.dtype:
                 raise ValueError(f"out is {out.dtype}, q {q.dtype}")
-            self._apart(q, out)
+            # every row's queries are read before its result is written: the two may be the same memory
+            if q.data_ptr() != out.data_ptr() or q.stride() != out.stride():
+                self._apart("q and out", q, out)
         rows = q.shape[0]
         batch, n, width, most = self._batch(table, "lengths", lengths, offsets, rows, most)
         if out is None:
@@ -176,19 +181,16 @@ class KVCache:
             raise ValueError(f"{name} with strides {t.stride()} cannot be written: adjacent features, no element twice")
 
     @staticmethod
-    def _apart(q, out):
-        """Every row's queries are read before its result is written, so the two may be the same memory; they may also lie side by
-        side in the rows of one tensor, but not overlap otherwise."""
-        if q.data_ptr() == out.data_ptr() and q.stride() == out.stride():
+    def _apart(names, a, b):
+        """Two tensors of a call may lie side by side in the rows of one, but not overlap."""
+        if a.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
             return
-        if q.numel() == 0 or q.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
-            return
-        reach = [1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) for t in (q, out)]
-        ahead = (out.data_ptr() - q.data_ptr()) // q.element_size()
+        reach = [1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) for t in (a, b)]
+        ahead = (b.data_ptr() - a.data_ptr()) // a.element_size()
         if ahead >= reach[0] or -ahead >= reach[1]:
             return
-        step = q.stride(0)
-        inner = [1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (q, out)]
-        if step == out.stride(0) and step > 0 and ahead % step >= inner[0] and step - ahead % step >= inner[1]:
+        step = a.stride(0)
+        inner = [1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (a, b)]
+        if step == b.stride(0) and step > 0 and ahead % step >= inner[0] and step - ahead % step >= inner[1]:
             return
-        raise ValueError("out shares memory with q")
+        raise ValueError(f"{names} share memory")
