@@ -246,54 +246,71 @@ def test_strides_alignment_and_in_place(dtype, count):
 
 
 # ---------------------------------------------------------------------------------------------------- large tiles
-# (what the sizes above do not reach: 128 rows a workgroup where the call is large enough)
+# (what the sizes above do not reach: 64 or 128 rows a workgroup, where a call is large enough)
 
-def batch_of(count, longest, most, seed):
-    g = torch.Generator().manual_seed(seed)
-    lengths = torch.randint(1, longest + 1, (count,), generator=g).tolist()
-    counts = [min(n, int(m)) for n, m in zip(lengths, torch.randint(0, most + 1, (count,), generator=g))]
+def tile_of(rows, sequences, most, longest, H, G, D, dtype, window=0, sinks=0):
+    return lib.vamd_kv_attend_tile(rows, sequences, most, longest, H, G, D, window, sinks, _lib.F32 if dtype == torch.float32 else _lib.BF16)
+
+
+def batch_of(tile, longest, most, H, G, D, dtype, even=False):
+    """Lengths and query counts of the smallest batch of this kind that is served by tiles of `tile` rows; unequal, one sequence
+    without queries, one that ends with a group, unless `even`."""
+    g = torch.Generator().manual_seed(D + G)
+    lengths = torch.randint(1, longest + 1, (400,), generator=g).tolist()
+    counts = [min(n, int(m)) for n, m in zip(lengths, torch.randint(0, most + 1, (400,), generator=g))]
     lengths[0], counts[0] = longest, most
     lengths[1], counts[1] = 64, min(64, most)
     counts[2] = 0
-    return lengths, counts
+    if even:
+        lengths, counts = [longest] * 400, [most] * 400
+    for n in range(4, 400):
+        if tile_of(sum(counts[:n]), n, most, longest, H, G, D, dtype) == tile:
+            return lengths[:n], counts[:n]
+    raise AssertionError("no such batch")
 
 
-def attend_large(c, q, table, lengths, counts, H, G, D, dtype, window=0, sinks=0, **kw):
-    t = _lib.F32 if dtype == torch.float32 else _lib.BF16
-    longest = max(lengths)
-    assert lib.vamd_kv_attend_tile(q.shape[0], len(lengths), max(counts), longest, H, G, D, window, sinks, t) == 128
-    return c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), most=max(counts), longest=longest, window=window, sinks=sinks, **kw)
+def attend_large(tile, c, q, table, lengths, counts, G, dtype, window=0, sinks=0, **kw):
+    longest, most = max(lengths), max(counts)
+    assert tile_of(q.shape[0], len(lengths), most, longest, c.kv_heads, G, c.head_dim, dtype, window, sinks) == tile
+    return c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), most=most, longest=longest, window=window, sinks=sinks, **kw)
 
 
+TILES = pytest.mark.parametrize("tile", [64, 128])
+
+
+@TILES
 @pytest.mark.parametrize("format", ["e4m3", "int8"])
 @pytest.mark.parametrize("dtype,D", [(torch.bfloat16, d) for d in (16, 32, 48, 64, 80, 96, 112, 128, 160, 176, 192, 224, 256)] +
                          [(torch.float32, d) for d in (16, 32, 48, 64, 80, 96, 112, 128)], ids=lambda x: str(x).replace("torch.", ""))
-def test_large_tiles(dtype, D, format):
-    H, G = (8, 1) if dtype == torch.bfloat16 else (16, 1)
-    lengths, counts = batch_of(24 if dtype == torch.bfloat16 else 34, 150, 130, D)
+def test_large_tiles(dtype, D, format, tile):
+    H = 16
+    lengths, counts = batch_of(tile, 150, 130, H, 1, D, dtype)
     c, table, k, v, off = filled(lengths, H, D, 64, format, 220)
-    q = rnd((sum(counts), H * G, D), dtype, 229)
-    compare(attend_large(c, q, table, lengths, counts, H, G, D, dtype), q, k, v, off, lengths, counts, D ** -0.5, dtype)
+    q = rnd((sum(counts), H, D), dtype, 229)
+    compare(attend_large(tile, c, q, table, lengths, counts, 1, dtype), q, k, v, off, lengths, counts, D ** -0.5, dtype)
 
 
+@TILES
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
 @pytest.mark.parametrize("group", [1, 3, 8])
-def test_large_tiles_groups_windows_and_edges(group, dtype):
-    H, D = (6, 64) if dtype == torch.bfloat16 else (12, 64)
-    lengths, counts = batch_of(30 if dtype == torch.bfloat16 else 50, 260, 90, group)
+def test_large_tiles_groups_windows_and_edges(group, dtype, tile):
+    H, D = 12, 64
+    lengths, counts = batch_of(tile, 260, 80, H, group, D, dtype)
     c, table, k, v, off = filled(lengths, H, D, 128, "e4m3", 240)
     n = sum(counts)
     q = rnd((n + 3, H * group, D), dtype, 249)
     out = torch.full_like(q, 7.0)
-    attend_large(c, q, table, lengths, counts, H, group, D, dtype, out=out)
+    attend_large(tile, c, q, table, lengths, counts, group, dtype, out=out)
     assert (out[n:] == 7).all()
     compare(out, q, k, v, off, lengths, counts, 0.125, dtype)
-    for window, sinks in ((1, 0), (64, 4), (100, 70), (1000, 3)):
-        compare(attend_large(c, q, table, lengths, counts, H, group, D, dtype, window, sinks), q, k, v, off, lengths, counts, 0.125, dtype,
+    for window, sinks in ((1, 0), (64, 4), (100, 70), (1000, 3)) if group < 8 else ((64, 4),):
+        compare(attend_large(tile, c, q, table, lengths, counts, group, dtype, window, sinks), q, k, v, off, lengths, counts, 0.125, dtype,
                 window=window, sinks=sinks)
-    compare(attend_large(c, q, table, lengths, counts, H, group, D, dtype, causal=False, scale=-0.2), q, k, v, off, lengths, counts, -0.2,
+    if group == 8:
+        return
+    compare(attend_large(tile, c, q, table, lengths, counts, group, dtype, causal=False, scale=-0.2), q, k, v, off, lengths, counts, -0.2,
             dtype, causal=False)
-    zero = attend_large(c, q, table, lengths, counts, H, group, D, dtype, scale=0.0)
+    zero = attend_large(tile, c, q, table, lengths, counts, group, dtype, scale=0.0)
     compare(zero, q, k, v, off, lengths, counts, 0.0, dtype)
     # more queries than tokens, lengths of zero, beyond the table and negative
     odd = [0, -3] + [2 ** 31 - 1 if i % 7 == 0 else max(1, n // 3) for i, n in enumerate(lengths[2:])]
@@ -303,17 +320,18 @@ def test_large_tiles_groups_windows_and_edges(group, dtype):
     compare(got, q, kr.cpu(), vr.cpu(), [room * b for b in range(len(odd) + 1)], [min(max(x, 0), room) for x in odd], counts, 0.125, dtype)
 
 
+@TILES
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
-def test_large_tiles_holes_and_what_is_not_finite(dtype):
-    H, G, D = (8, 2, 32) if dtype == torch.bfloat16 else (16, 2, 32)
-    count = 20 if dtype == torch.bfloat16 else 34
-    lengths, counts = [300] * count, [40] * count
+def test_large_tiles_holes_and_what_is_not_finite(dtype, tile):
+    H, G, D = 16, 2, 32
+    lengths, counts = batch_of(tile, 300, 40, H, G, D, dtype, even=True)
+    count = len(lengths)
     c, table, k, v, off = filled(lengths, H, D, 64, "e4m3", 260)
     q = rnd((40 * count, H * G, D), dtype, 269)
-    clean = attend_large(c, q, table, lengths, counts, H, G, D, dtype, window=72, sinks=3)
+    clean = attend_large(tile, c, q, table, lengths, counts, G, dtype, window=72, sinks=3)
     bad = torch.full((1, H, D), math.nan, device=DEV)
     c.append(bad, bad, table[:1], i32([200]))                 # block 3 (tokens 192 .. 255) of sequence 0
-    out = attend_large(c, q, table, lengths, counts, H, G, D, dtype, window=72, sinks=3)
+    out = attend_large(tile, c, q, table, lengths, counts, G, dtype, window=72, sinks=3)
     assert torch.equal(out[40:], clean[40:])
     for i in range(40):                                       # query 260 + i sees tokens from 189 + i on
         assert torch.isnan(out[i]).all() if 189 + i < 256 else torch.equal(out[i], clean[i]), i
@@ -321,82 +339,88 @@ def test_large_tiles_holes_and_what_is_not_finite(dtype):
     table[0, 3], table[1, 0], table[2, 4], table[3] = -1, c.blocks, 2 ** 31 - 1, -5
     holes = [torch.zeros(320, dtype=torch.bool) for _ in lengths]
     holes[0][192:256] = holes[1][:64] = holes[2][256:] = holes[3][:] = True
-    out = attend_large(c, q, table, lengths, counts, H, G, D, dtype)
+    out = attend_large(tile, c, q, table, lengths, counts, G, dtype)
     compare(out, q, k, v, off, lengths, counts, 32 ** -0.5, dtype, holes=holes)
     assert (out[120:160] == 0).all()
 
 
-def test_large_tiles_values_of_any_scale():
-    """Values' scales far from 1 (they go into the probabilities' exponent while that is safe), zero blocks, blocks of unlike scale."""
-    H, D, count = 8, 32, 20
-    for dtype in DTYPES:
-        n = count if dtype == torch.bfloat16 else 70
-        lengths, counts = [256] * n, [70] * n
-        c = KVCache(4 * n, H, D, device=DEV)
-        table = torch.arange(4 * n, dtype=torch.int32, device=DEV).view(n, 4)
-        k, v = rnd((256 * n, H, D), torch.float32, 1), rnd((256 * n, H, D), torch.float32, 2).view(n, 4, 64, H, D)
-        for b in range(n):
-            for i in range(4):
-                v[b, i] *= (2.0 ** -90, 2.0 ** 60, 0.0, 1.0, 2.0 ** -45, 2.0 ** 45, 2.0 ** 100)[(b + 3 * i) % 7] if b else (0.0, 1.0, 0.0, 2.0 ** -100)[i]
-        c.append(k, v.view(-1, H, D), table, i32([0] * n))
-        kb, vb = c.read(table, i32([0] * n), 256 * n, dtype=torch.float32)
-        q = rnd((70 * n, H, D), dtype, 3)
-        out = attend_large(c, q, table, lengths, counts, H, 1, D, dtype)
-        compare(out, q, kb.cpu(), vb.cpu(), [256 * b for b in range(n + 1)], lengths, counts, D ** -0.5, dtype)
-
-
+@TILES
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
-def test_large_tiles_split_and_joined(dtype):
-    H, G, D = (8, 2, 64) if dtype == torch.bfloat16 else (20, 2, 64)
-    lengths, counts = [6100, 3000, 40, 1500, 5000, 700], [40, 64, 40, 1, 33, 0]
+def test_large_tiles_values_of_any_scale(dtype, tile):
+    """Values' scales far from 1 (they go into the probabilities' exponent while that is safe), zero blocks, blocks of unlike scale."""
+    H, D = 16, 32
+    lengths, counts = batch_of(tile, 256, 70, H, 1, D, dtype, even=True)
+    n = len(lengths)
+    c = KVCache(4 * n, H, D, device=DEV)
+    table = torch.arange(4 * n, dtype=torch.int32, device=DEV).view(n, 4)
+    k, v = rnd((256 * n, H, D), torch.float32, 1), rnd((256 * n, H, D), torch.float32, 2).view(n, 4, 64, H, D)
+    for b in range(n):
+        for i in range(4):
+            v[b, i] *= (2.0 ** -90, 2.0 ** 60, 0.0, 1.0, 2.0 ** -45, 2.0 ** 45, 2.0 ** 100)[(b + 3 * i) % 7] if b else (0.0, 1.0, 0.0, 2.0 ** -100)[i]
+    c.append(k, v.view(-1, H, D), table, i32([0] * n))
+    kb, vb = c.read(table, i32([0] * n), 256 * n, dtype=torch.float32)
+    q = rnd((70 * n, H, D), dtype, 3)
+    out = attend_large(tile, c, q, table, lengths, counts, 1, dtype)
+    compare(out, q, kb.cpu(), vb.cpu(), [256 * b for b in range(n + 1)], lengths, counts, D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("tile,longest", [(64, 11000), (128, 16000)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
+def test_large_tiles_split_and_joined(dtype, tile, longest):
+    H, G, D = 8, 2, 64
+    lengths, counts = [longest, 9000, 40, 1500, 5000, 700], [40, 64, 40, 1, 33, 0]
     c, table, k, v, off = filled(lengths, H, D, 64, "int8", 280)
     q = rnd((sum(counts), H * G, D), dtype, 289)
     t = _lib.F32 if dtype == torch.float32 else _lib.BF16
-    assert lib.vamd_kv_attend_workspace(sum(counts), 6, 64, 6100, H, G, D, 0, 0, t) > 0
-    compare(attend_large(c, q, table, lengths, counts, H, G, D, dtype), q, k, v, off, lengths, counts, 0.125, dtype)
-    compare(attend_large(c, q, table, lengths, counts, H, G, D, dtype, 5000, 70), q, k, v, off, lengths, counts, 0.125, dtype, window=5000,
+    assert lib.vamd_kv_attend_workspace(sum(counts), 6, 64, longest, H, G, D, 0, 0, t) > 0
+    compare(attend_large(tile, c, q, table, lengths, counts, G, dtype), q, k, v, off, lengths, counts, 0.125, dtype)
+    compare(attend_large(tile, c, q, table, lengths, counts, G, dtype, longest - 100, 70), q, k, v, off, lengths, counts, 0.125, dtype, window=longest - 100,
             sinks=70)
-    want = attend_large(c, q, table, lengths, counts, H, G, D, dtype)
+    want = attend_large(tile, c, q, table, lengths, counts, G, dtype)
     g = torch.cuda.CUDAGraph()
     n, o = i32(lengths), i32(offsets_of(counts))
     with torch.cuda.graph(g):
-        got = c.attend(q, table, n, offsets=o, most=64, longest=6100)
+        got = c.attend(q, table, n, offsets=o, most=64, longest=longest)
     for step in range(3):
         g.replay()
-        assert torch.equal(c.attend(q, table, n, offsets=o, most=64, longest=6100), want)
+        assert torch.equal(c.attend(q, table, n, offsets=o, most=64, longest=longest), want)
         torch.cuda.synchronize()
         assert torch.equal(got, want), step
 
 
+@TILES
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
-def test_large_tiles_strides_and_in_place(dtype):
-    H, G, D = (8, 1, 48) if dtype == torch.bfloat16 else (16, 1, 48)
-    count = 20 if dtype == torch.bfloat16 else 34
-    lengths, counts = [90] * count, [70] * count
+def test_large_tiles_strides_and_in_place(dtype, tile):
+    H, D = 16, 48
+    lengths, counts = batch_of(tile, 90, 70, H, 1, D, dtype, even=True)
     c, table, k, v, off = filled(lengths, H, D, 64, "e4m3", 300)
-    n = 70 * count
+    n = sum(counts)
     q = rnd((n, H, D), dtype, 309)
-    want = attend_large(c, q, table, lengths, counts, H, G, D, dtype)
+    want = attend_large(tile, c, q, table, lengths, counts, 1, dtype)
+    compare(want, q, k, v, off, lengths, counts, D ** -0.5, dtype)
     fused = torch.zeros((n, 2 * H * D + 1), dtype=dtype, device=DEV)
     view, out = fused[:, 1:1 + H * D].unflatten(1, (H, D)), fused[:, 1 + H * D:].unflatten(1, (H, D))
     view.copy_(q)
-    c.attend(view, table, i32(lengths), out=out)
+    c.attend(view, table, i32(lengths), longest=90, out=out)
     assert torch.equal(out, want) and torch.equal(view, q)
     heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
-    assert torch.equal(c.attend(heads_first, table, i32(lengths)), want)
+    assert torch.equal(c.attend(heads_first, table, i32(lengths), longest=90), want)
     same = q.clone()
-    assert c.attend(same, table, i32(lengths), out=same) is same and torch.equal(same, want)
+    assert c.attend(same, table, i32(lengths), longest=90, out=same) is same and torch.equal(same, want)
 
 
-def test_many_sequences():
-    """More sequences than a wave has lanes: whose tile a workgroup takes is found 64 sequences at a time."""
-    count, H, D = 150, 2, 32
+@pytest.mark.parametrize("H,most", [(1, 80), (2, 80), (4, 80), (2, 20)])
+def test_many_sequences(H, most):
+    """More sequences than a wave has lanes: whose tile a workgroup takes is found 64 sequences at a time; tiles of any size."""
+    count, D = 150, 32
     lengths = [1 + (37 * i) % 90 for i in range(count)]
-    counts = [0 if i % 5 == 0 else min(n, 1 + (i * 13) % 80) for i, n in enumerate(lengths)]
-    counts[149], lengths[149] = 70, 90
+    counts = [0 if i % 5 == 0 else min(n, 1 + (i * 13) % most) for i, n in enumerate(lengths)]
+    counts[149], lengths[149] = most, 90
     c, table, k, v, off = filled(lengths, H, D, 64, "e4m3", 320)
     q = rnd((sum(counts), H, D), torch.bfloat16, 329)
-    compare(attend_large(c, q, table, lengths, counts, H, 1, D, torch.bfloat16), q, k, v, off, lengths, counts, D ** -0.5, torch.bfloat16)
+    assert tile_of(sum(counts), count, most, 90, H, 1, D, torch.bfloat16) == {(1, 80): 16, (2, 80): 64, (4, 80): 128, (2, 20): 16}[H, most]
+    out = c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), most=most, longest=90)
+    compare(out, q, k, v, off, lengths, counts, D ** -0.5, torch.bfloat16)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
@@ -407,8 +431,7 @@ def test_rows_beyond_most_are_left_out(dtype, sequences, H):
     c, table, k, v, off = filled(lengths, H, 32, 64, "e4m3", 340)
     o = offsets_of(counts)
     q = rnd((o[-1], H, 32), dtype, 349)
-    t = _lib.F32 if dtype == torch.float32 else _lib.BF16
-    assert lib.vamd_kv_attend_tile(o[-1], sequences, most, 200, H, 1, 32, 0, 0, t) == (16 if sequences == 3 else 128)
+    assert tile_of(o[-1], sequences, most, 200, H, 1, 32, dtype) == (16 if sequences == 3 else 128)
     want = c.attend(q, table, i32(lengths), offsets=i32(o), most=max(counts), longest=200)
     got = c.attend(q, table, i32(lengths), offsets=i32(o), most=most, longest=200, out=torch.full_like(q, 7.0))
     compare(want, q, k, v, off, lengths, counts, 32 ** -0.5, dtype)

@@ -37,7 +37,7 @@ struct KvAttendArgs {
     float* part;                 // [tile rows][splits][D] outputs, then [tile rows][splits][2] maximum and sum
     float* part_ml;
     float scale2;                // scale * log2(e)
-    int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, tile_rows, splits, q_aligned, o_aligned;
+    int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, all_tiles, tile_rows, splits, q_aligned, o_aligned;
 };
 
 // Groups of 64 tokens that the rows of a tile can see: `sink_groups` from 0 on, then those from `first` on; `count` in all.
@@ -70,6 +70,38 @@ __device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
     int n = a.lengths[b];
     n = n < 0 ? 0 : n;
     return n > room ? (int)room : n;
+}
+
+// Whose is tile number `tile` among those that the sequences really have, one sequence after the other?  Gives the sequence and the tile's
+// number in it, or false behind the last one.  64 sequences at a time, by the whole wave.
+//
+// Walked over by `most` instead, the tiles that short sequences do not have lie between the others in a regular pattern that leaves
+// whole CUs idle: prompts of 4096 and 925 tokens 435 us, of 4096 alone 264.
+__device__ __forceinline__ bool kv_whose_tile(const KvAttendArgs& a, int lane, int& tile, int& b) {
+    if (!a.offsets || a.tiles == 1) {
+        b = tile / a.tiles;
+        tile -= b * a.tiles;
+        return b < a.sequences;
+    }
+    for (int b0 = 0; b0 < a.sequences; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < a.sequences) n = (kv_rows(a.offsets, b0 + lane, a.rows, a.most).count * a.group + a.tile_rows - 1) / a.tile_rows;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(upto, o, 64);
+            upto += lane >= o ? t : 0;
+        }
+        const uint64_t behind = __ballot(upto > tile);
+        if (behind) {
+            const int l = __ffsll((unsigned long long)behind) - 1;
+            b = __builtin_amdgcn_readfirstlane(b0 + l);
+            tile = __builtin_amdgcn_readfirstlane(tile - __shfl(upto - n, l, 64));
+            return true;
+        }
+        tile -= __shfl(upto, 63, 64);
+    }
+    return false;
 }
 
 __device__ __forceinline__ float kv_over_groups_max(float v) {           // over the four lanes that hold one query's keys
@@ -105,14 +137,16 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    // heads and sequences vary fastest, shares slowest: workgroups without work (shares that a short sequence does not have) then
-    // sit behind each other and not on every second XCD or CU
+    // Heads vary fastest, then the tiles, shares slowest: workgroups without work (shares that a short sequence does not have) then sit
+    // behind each other and not on every second XCD or CU.
     uint32_t id = blockIdx.x;
-    const uint32_t pairs = (uint32_t)a.sequences * a.heads, pair = id % pairs;
-    id /= pairs;
-    const int tile = (int)(id % (uint32_t)a.tiles), split = (int)(id / (uint32_t)a.tiles);
-    const int h = (int)(pair % (uint32_t)a.heads), b = (int)(pair / (uint32_t)a.heads);
-    const int64_t slot = ((int64_t)pair * a.tiles + tile) * 16;
+    const int h = (int)(id % (uint32_t)a.heads);
+    id /= (uint32_t)a.heads;
+    const uint32_t tiles = (uint32_t)a.all_tiles;
+    const int split = (int)(id / tiles);
+    int tile = (int)(id % tiles), b;
+    if (!kv_whose_tile(a, lane, tile, b)) return;
+    const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * 16;
 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     if (tile * 16 >= rows.count * a.group) return;
@@ -374,13 +408,19 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 
 // ---------------------------------------------------------------------------------------------------- many queries (prompts)
 //
-// A workgroup of four waves takes 128 * CB rows, a wave 32 * CB of them as the columns of v_mfma_f32_32x32x16_bf16, and walks over the
-// keys 64 at a time.  The codes of a group become bf16 ONCE per workgroup on their way into LDS (both operands in the
-// order in which the products read them, 16 bytes a lane, no bank conflicts; the next group's codes are in flight meanwhile and
-// go to the other buffer behind the products, one barrier a group).  A lane ends up with 16 scores of one query per 32 keys,
-// again in the slots in which the second product wants the probabilities: the row maximum needs one exchange between two lanes.
-// The running maximum is a reference that moves only when a score exceeds it by 2^8 or more (probabilities up to 256 are as exact
-// as below 1), so that the outputs are hardly ever rescaled.  The values' power-of-two scale goes into the exponent.
+// A workgroup of four waves takes 128 rows, a wave 32 of them as the columns of v_mfma_f32_32x32x16_bf16, and walks over the keys 64 at
+// a time (KW = 1); or 64 rows, two waves on each half of the keys (KW = 2), whose results meet in LDS at the end: half
+// the time for a tile where there are few of them.  The codes of a group become bf16 ONCE per workgroup on their way into LDS (both
+// operands in the order in which the products read them, 16 bytes a lane, no bank conflicts; the next group's codes are in
+// flight meanwhile and go to the other buffer behind the products, one barrier a group).  A lane ends up with 16 scores of
+// one query per 32 keys, again in the slots in which the second product wants the probabilities: the row maximum needs
+// one exchange between two lanes.  The running maximum is a reference that moves only when a score exceeds it by 2^8 or more
+// (probabilities up to 256 are as exact as below 1), so that the outputs are hardly ever rescaled.  The values' power-of-two
+// scale goes into the exponent.
+//
+// Bound by the matrix cores, the exponentials and the LDS reads about alike (an operand is read once for 32 queries, 128 bytes a
+// clock): 30000 keys before 2048 queries of 32 heads, 128 features, 936 TFLOP/s; prompts of 4096 and 925 tokens behind
+// 1000 780, where causal tiles of unlike length leave some of the chip idle; a plain bf16 product of 8192^3 reaches 1234.
 //
 // DT: tiles of 32 features (the last may be half empty).
 __device__ __forceinline__ float kv_over_halves_max(float v) {               // over the two lanes that hold one query's keys
@@ -392,52 +432,25 @@ __device__ __forceinline__ float kv_over_halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-constexpr int kKvTileThreads = 256, kKvTileRows = 128;
+constexpr int kKvTileThreads = 256;
 
-template <typename T, int FMT, int DT, int CB>
+template <typename T, int FMT, int DT, int KW>
 __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4) ? 2 : 1) kv_attend_tile_kernel(const KvAttendArgs a) {
     constexpr int N = sizeof(T) == 4 ? 3 : 1;
     constexpr int PIECES = (DT * 2 * 64 + kKvTileThreads - 1) / kKvTileThreads;      // 16-byte pieces of a group a thread stages
     constexpr int KBYTES = DT * 4 * 64 * 16, BUF = 2 * KBYTES;
+    constexpr int KH = 2 / KW, ROW_WAVES = 4 / KW;                           // halves of a group's keys a wave takes; waves over the rows
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 31, hh = lane >> 5;
-    // Heads vary fastest (where they are a multiple of 8 the tiles of one meet in one XCD's L2), then the shares, then the tiles that
-    // the sequences really have, one sequence after the other, late ones (the longest, where queries are causal) first.  Walked over by
-    // `most` instead, tiles that short sequences do not have lie between the others in a regular pattern that leaves whole
-    // CUs idle: prompts of 4096 and 925 tokens 435 us, of 4096 alone 264.
+    const int c = lane & 31, hh = lane >> 5, wave_r = wave % ROW_WAVES, kh0 = wave / ROW_WAVES;
+    // Heads vary fastest (where they are a multiple of 8 the tiles of one meet in one XCD's L2), then the shares, then the tiles, late
+    // ones of a sequence (the longest, where queries are causal) first.
     uint32_t id = blockIdx.x;
     const int h = (int)(id % (uint32_t)a.heads);
     id /= (uint32_t)a.heads;
     const int split = (int)(id % (uint32_t)a.splits);
-    int tile = (int)(id / (uint32_t)a.splits), b = 0;
-    if (!a.offsets) {
-        b = tile / a.tiles;
-        tile -= b * a.tiles;
-    } else {
-        for (int b0 = 0;; b0 += 64) {                        // 64 sequences at a time: whose tile is it?
-            if (b0 >= a.sequences) return;
-            const int mine = b0 + lane;
-            int n = 0;
-            if (mine < a.sequences) n = (kv_rows(a.offsets, mine, a.rows, a.most).count * a.group + a.tile_rows - 1) / a.tile_rows;
-            int upto = n;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int t = __shfl_up(upto, o, 64);
-                upto += lane >= o ? t : 0;
-            }
-            const uint64_t behind = __ballot(upto > tile);
-            if (behind) {
-                const int l = __ffsll((unsigned long long)behind) - 1;
-                b = b0 + l;
-                tile -= __shfl(upto - n, l, 64);
-                break;
-            }
-            tile -= __shfl(upto, 63, 64);
-        }
-        b = __builtin_amdgcn_readfirstlane(b);
-        tile = __builtin_amdgcn_readfirstlane(tile);
-    }
+    int tile = (int)(id / (uint32_t)a.splits), b;
+    if (!kv_whose_tile(a, lane, tile, b)) return;
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int all_rows = rows.count * a.group;
     tile = (all_rows + a.tile_rows - 1) / a.tile_rows - 1 - tile;
@@ -515,24 +528,18 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         entry = entry_of(begin);
         fetch(begin);
     }
-    // queries: column c of block cb is row first_row + (wave * CB + cb) * 32 + c
-    kv_bf16x8 qf[CB][N][DT * 2];
-    int tok[CB], head[CB], upto[CB], from[CB];
-    bool live[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const int row = first_row + (wave * CB + cb) * 32 + c;
-        tok[cb] = row / a.group;
-        head[cb] = h * a.group + row - tok[cb] * a.group;
-        live[cb] = tok[cb] < rows.count;
-        const int pos = a.causal ? shift + tok[cb] : length - 1;
-        upto[cb] = pos < length ? pos : length - 1;
-        from[cb] = a.window > 0 ? pos - a.window + 1 : 0;
-        const T* q = (const T*)a.q + (rows.first + (live[cb] ? tok[cb] : 0)) * a.q_tok + head[cb] * a.q_head;
+    // queries: column c is row first_row + 32 wave_r + c
+    const int row = first_row + wave_r * 32 + c, tok = row / a.group, head = h * a.group + row - tok * a.group;
+    const bool live = tok < rows.count;
+    const int pos = a.causal ? shift + tok : length - 1;
+    const int upto = pos < length ? pos : length - 1, from = a.window > 0 ? pos - a.window + 1 : 0, first_keys = a.window > 0 ? a.sinks : 0;
+    kv_bf16x8 qf[N][DT * 2];
+    {
+        const T* q = (const T*)a.q + (rows.first + (live ? tok : 0)) * a.q_tok + head * a.q_head;
 #pragma unroll
         for (int k = 0; k < DT * 2; ++k) {
             T v[8] = {};
-            if (live[cb] && k < S) {
+            if (live && k < S) {
                 const T* p = q + k * 16 + hh * 8;
                 if (a.q_aligned) {
 #pragma unroll
@@ -544,28 +551,22 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if constexpr (N == 1) qf[cb][0][k][e] = v[e];
+                if constexpr (N == 1) qf[0][k][e] = v[e];
                 else {
                     bf16_t p[N];
                     kv_pieces<N>(v[e], p);
 #pragma unroll
-                    for (int n = 0; n < N; ++n) qf[cb][n][k][e] = p[n];
+                    for (int n = 0; n < N; ++n) qf[n][k][e] = p[n];
                 }
             }
         }
     }
-    const int first_keys = a.window > 0 ? a.sinks : 0;
-    kv_f32x16 acc[CB][DT];
-    float m[CB], l[CB];
+    kv_f32x16 acc[DT];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        m[cb] = -INFINITY;
-        l[cb] = 0.f;
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[cb][t][i] = 0.f;
-    }
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
     if (begin < end) {
         // keys' slabs that the head does not have are zero in both buffers (values' rows there end up in outputs that nobody reads)
         for (int q = S * 128 + tid; q < DT * 2 * 128; q += kKvTileThreads) {
@@ -585,29 +586,27 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         const unsigned char* kb = smem + buf * BUF;
         const unsigned char* vb = kb + KBYTES;
         // operands are read in batches of R, one batch ahead of the products
-        constexpr int R = DT % 2 ? 2 : 4, BATCHES = DT * 4 / R;
+        constexpr int READS = KH * 2 * DT, R = READS % 4 ? 2 : 4, BATCHES = READS / R;
         kv_bf16x8 fr[2][R];
-        auto read_k = [&](int i) {                           // batch i: keys 32 kh + c, features 16 k + 8 hh ..
+        auto read_k = [&](int i) {                           // batch i: keys 32 (kh0 + kh) + c, features 16 k + 8 hh ..
 #pragma unroll
             for (int e = 0; e < R; ++e) {
                 const int kh = (i * R + e) / (DT * 2), k = (i * R + e) % (DT * 2);
-                fr[i & 1][e] = *(const kv_bf16x8*)(kb + ((k * 2 + hh) * 64 + kh * 32 + c) * 16);
+                fr[i & 1][e] = *(const kv_bf16x8*)(kb + ((k * 2 + hh) * 64 + (kh0 + kh) * 32 + c) * 16);
             }
         };
         auto read_v = [&](int i) {                           // batch i: feature 32 t + c, tokens of step s and half hh
 #pragma unroll
             for (int e = 0; e < R; ++e) {
                 const int s = (i * R + e) / DT, t = (i * R + e) % DT;
-                fr[i & 1][e] = *(const kv_bf16x8*)(vb + ((s * 2 + hh) * (DT * 32) + t * 32 + c) * 16);
+                fr[i & 1][e] = *(const kv_bf16x8*)(vb + (((kh0 * 2 + s) * 2 + hh) * (DT * 32) + t * 32 + c) * 16);
             }
         };
-        kv_f32x16 sc[CB][2];
+        kv_f32x16 sc[KH];
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
+        for (int kh = 0; kh < KH; ++kh)
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[cb][kh][i] = 0.f;
+            for (int i = 0; i < 16; ++i) sc[kh][i] = 0.f;
         read_k(0);
 #pragma unroll
         for (int i = 0; i < BATCHES; ++i) {
@@ -616,10 +615,7 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
             for (int e = 0; e < R; ++e) {
                 const int kh = (i * R + e) / (DT * 2), k = (i * R + e) % (DT * 2);
 #pragma unroll
-                for (int n = N - 1; n >= 0; --n)
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        sc[cb][kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], qf[cb][n][k], sc[cb][kh], 0, 0, 0);
+                for (int n = N - 1; n >= 0; --n) sc[kh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], qf[n][k], sc[kh], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -629,11 +625,9 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         const float f = by_hand ? 1.f : f_raw;
         if (by_hand) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
+            for (int kh = 0; kh < KH; ++kh)
 #pragma unroll
-                for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[cb][kh][i] *= f_raw;
+                for (int i = 0; i < 16; ++i) sc[kh][i] *= f_raw;
         }
         const bool edge = page < 0 || k0 + kKvGroup > p_first + 1 || k0 + kKvGroup > length ||
                           (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
@@ -641,68 +635,65 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         const int v_exp = (int)(__float_as_uint(v_scale) >> 23) - 127;
         const bool fold = v_exp >= -40 && v_exp <= 40;
         const float v_add = fold ? (float)v_exp : 0.f, v_undo = fold ? __uint_as_float((uint32_t)(127 - v_exp) << 23) : 1.f;
-        kv_bf16x8 pf[CB][N][4];
+        const int k1 = k0 + kh0 * 32 + hh * 4;               // token of the lane's first score
+        if (edge) {
+            const int rel_upto = page < 0 ? -1 : upto - k1, rel_from = from - k1, rel_first = first_keys - k1;
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            if (edge) {
-                const int k1 = k0 + hh * 4;
-                const int rel_upto = page < 0 ? -1 : upto[cb] - k1, rel_from = from[cb] - k1, rel_first = first_keys - k1;
-#pragma unroll
-                for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = kh * 32 + (i >> 2) * 8 + (i & 3);
-                        const bool seen = j <= rel_upto && (j >= rel_from || j < rel_first);
-                        sc[cb][kh][i] = seen ? sc[cb][kh][i] : -INFINITY;
-                    }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[cb][kh][i]);
-            top = kv_over_halves_max(top) * f;
-            if (__any(top > m[cb] + 8.f)) {
-                const float m_new = top > m[cb] + 8.f ? top : m[cb];
-                const float alpha = __builtin_amdgcn_exp2f(m[cb] - kv_finite(m_new));
-                l[cb] *= alpha;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[cb][t][i] *= alpha;
-                m[cb] = m_new;
-            }
-            const float shift_by = v_add - kv_finite(m[cb]);
-            float sum = 0.f;
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
+            for (int kh = 0; kh < KH; ++kh)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[cb][kh][i], f, shift_by));
-                    sum += e;
-                    sc[cb][kh][i] = e;
-                }
-            l[cb] = fmaf(sum, v_undo, l[cb]);
-            if (!fold) {                                     // NaN: only to the queries that see the block
-#pragma unroll
-                for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = k0 + hh * 4 + kh * 32 + (i >> 2) * 8 + (i & 3);
-                        const bool seen = page >= 0 && j <= upto[cb] && (j >= from[cb] || j < first_keys);
-                        sc[cb][kh][i] = seen ? sc[cb][kh][i] * v_scale : 0.f;
-                    }
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    bf16_t p[N];
-                    kv_pieces<N>(sc[cb][s >> 1][(s & 1) * 8 + e], p);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) pf[cb][n][s][e] = p[n];
+                    const int j = kh * 32 + (i >> 2) * 8 + (i & 3);
+                    const bool seen = j <= rel_upto && (j >= rel_from || j < rel_first);
+                    sc[kh][i] = seen ? sc[kh][i] : -INFINITY;
                 }
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kh][i]);
+        top = kv_over_halves_max(top) * f;
+        if (__any(top > m + 8.f)) {
+            const float m_new = top > m + 8.f ? top : m;
+            const float alpha = __builtin_amdgcn_exp2f(m - kv_finite(m_new));
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+            m = m_new;
+        }
+        const float shift_by = v_add - kv_finite(m);
+        float sum = 0.f;
+#pragma unroll
+        for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(sc[kh][i], f, shift_by));
+                sum += e;
+                sc[kh][i] = e;
+            }
+        l = fmaf(sum, v_undo, l);
+        if (!fold) {                                         // NaN: only to the queries that see the block
+#pragma unroll
+            for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = k1 + kh * 32 + (i >> 2) * 8 + (i & 3);
+                    const bool seen = page >= 0 && j <= upto && (j >= from || j < first_keys);
+                    sc[kh][i] = seen ? sc[kh][i] * v_scale : 0.f;
+                }
+        }
+        kv_bf16x8 pf[N][2 * KH];
+#pragma unroll
+        for (int s = 0; s < 2 * KH; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16_t p[N];
+                kv_pieces<N>(sc[s >> 1][(s & 1) * 8 + e], p);
+#pragma unroll
+                for (int n = 0; n < N; ++n) pf[n][s][e] = p[n];
+            }
 #pragma unroll
         for (int i = 0; i < BATCHES; ++i) {
             if (i + 1 < BATCHES) read_v(i + 1);
@@ -710,54 +701,71 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
             for (int e = 0; e < R; ++e) {
                 const int s = (i * R + e) / DT, t = (i * R + e) % DT;
 #pragma unroll
-                for (int n = N - 1; n >= 0; --n)
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        acc[cb][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], pf[cb][n][s], acc[cb][t], 0, 0, 0);
+                for (int n = N - 1; n >= 0; --n) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[i & 1][e], pf[n][s], acc[t], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if (more) stage(buf ^ 1);
     }
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const float total = kv_over_halves_sum(l[cb]);
-        if (!live[cb]) continue;
-        if (a.splits > 1) {
-            const int64_t at = (slot + (wave * CB + cb) * 32 + c) * a.splits + split;
-            float* part = a.part + at * a.D;
+    float total = kv_over_halves_sum(l);
+    if constexpr (KW == 2) {
+        // the waves of the keys' second halves hand theirs to those of the first: [wave_r][register][lane]
+        __syncthreads();
+        float* box = (float*)smem + wave_r * (DT * 16 + 2) * 64 + lane;
+        if (kh0 == 1) {
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (t * 2 + (i >> 1) < S)
-                        *(kv_f32x4*)(part + t * 32 + i * 8 + hh * 4) = kv_f32x4{acc[cb][t][4 * i], acc[cb][t][4 * i + 1], acc[cb][t][4 * i + 2], acc[cb][t][4 * i + 3]};
-            if (hh == 0) {
-                a.part_ml[at * 2] = m[cb];
-                a.part_ml[at * 2 + 1] = total;
-            }
-            continue;
+                for (int i = 0; i < 16; ++i) box[(t * 16 + i) * 64] = acc[t][i];
+            box[DT * 16 * 64] = m;
+            box[(DT * 16 + 1) * 64] = total;
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        T* o = (T*)a.o + (rows.first + tok[cb]) * a.o_tok + head[cb] * a.o_head;
+        __syncthreads();
+        if (kh0 == 1) return;
+        const float m2 = box[DT * 16 * 64], m_new = fmaxf(m, m2);
+        const float f1 = __builtin_amdgcn_exp2f(m - kv_finite(m_new)), f2 = __builtin_amdgcn_exp2f(m2 - kv_finite(m_new));
+        m = m_new;
+        total = total * f1 + box[(DT * 16 + 1) * 64] * f2;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t * 2 + (i >> 1) >= S) continue;
-                T v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = from_f<T>(acc[cb][t][4 * i + e] * inv);
-                T* to = o + t * 32 + i * 8 + hh * 4;
-                if (a.o_aligned) {
-                    if (sizeof(T) == 4) *(kv_u32x4*)to = *(const kv_u32x4*)v;
-                    else *(kv_u32x2*)to = *(const kv_u32x2*)v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = v[e];
-                }
-            }
+            for (int i = 0; i < 16; ++i) acc[t][i] = acc[t][i] * f1 + box[(t * 16 + i) * 64] * f2;
     }
+    if (!live) return;
+    if (a.splits > 1) {
+        const int64_t at = (slot + wave_r * 32 + c) * a.splits + split;
+        float* part = a.part + at * a.D;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t * 2 + (i >> 1) < S)
+                    *(kv_f32x4*)(part + t * 32 + i * 8 + hh * 4) = kv_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+        if (hh == 0) {
+            a.part_ml[at * 2] = m;
+            a.part_ml[at * 2 + 1] = total;
+        }
+        return;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    T* o = (T*)a.o + (rows.first + tok) * a.o_tok + head * a.o_head;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (t * 2 + (i >> 1) >= S) continue;
+            T v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = from_f<T>(acc[t][4 * i + e] * inv);
+            T* to = o + t * 32 + i * 8 + hh * 4;
+            if (a.o_aligned) {
+                if (sizeof(T) == 4) *(kv_u32x4*)to = *(const kv_u32x4*)v;
+                else *(kv_u32x2*)to = *(const kv_u32x2*)v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[e] = v[e];
+            }
+        }
 }
 
 // Joins the shares of a row: one workgroup of 16 waves per row.  The shares' weights go to LDS first, so that the loads of the
@@ -828,14 +836,18 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     }
 }
 
-// How a call is cut.  Tiles of 16 rows of a (sequence, key head), or of 128 where these are enough to fill the chip: the
-// large tiles take four times the queries through a CU (8000 keys, 4 x 1024 queries of 32 heads: 242 us against 1063), but a chip
-// has room for 512 of them.  Measured with 8 key heads and 128 features: 512 queries, 128 large tiles, 27 us either way; 100
-// queries, 32 tiles, 18 us with large ones against 11; 16 x 200 queries of 12 heads, 384 tiles, 19 against 23.  float32 takes three
-// products: 4 x 512 queries of 16 heads 106 us with large tiles against 80, 2 x 2000 of 32 heads 260 against 316.
-// Then shares of the keys so that 512 workgroups (two a CU, all resident) have work, none of them less than 8 groups of 64 tokens (16
-// for large tiles).  One token of 64 sequences of up to 4096 (8 key heads, 128 features): 61 us with 256 or 512, 70 with 768 and
-// 68 with 1024 workgroups; of one sequence of 131071: 40, 42, 44 and 45 us.
+// How a call is cut.
+//
+// Tiles of 16 rows of a (sequence, key head), or of 128 or 64 where these are enough to fill the chip, which has room for 512 (for more
+// than 128 features 256) workgroups of them: 128 rows from 512 workgroups on, 64 above 256.  us with 8 key heads of 128 features
+// and groups of 4 (16 / 64 / 128 rows): 2048 queries (512 tiles of 128) 150 / 92 / 75; up to 4 x 1024 behind 8000 keys 355 / 255 / 240; 4096
+// queries of 8 ungrouped heads of 64 features 84 / 71 / 86; 512 queries (128 tiles) 30 / 24 / 28; 16 x 30 behind 1000 (128) 26 / 34 / 41; 100
+// queries (32) 14 / 17 / 18.  float32 (three products): up to 2 x 2000 queries 202 / 218 / 163, up to 4 x 200 30 / 39 / 51.
+//
+// Then shares of the keys, until 512 workgroups have work.  Tiles of 16: no share less than 8 groups of 64 tokens.  One token of
+// 64 sequences of up to 4096 (8 key heads, 128 features): 61 us with 256 or 512, 70 with 768 and 68 with 1024 workgroups; of
+// one sequence of 131071: 40, 42, 44 and 45 us.  Large tiles, whose partial results are many: only from 4 shares of 16 groups on
+// (2048 queries as two shares 140 us, as one 71; 64 queries behind 60000 keys as 32 shares 104).
 struct KvPlan {
     int tile_rows, tiles, splits;    // tiles of a sequence of `most` rows
     int64_t slots, grid;
@@ -846,23 +858,23 @@ static KvPlan kv_plan(int64_t all_rows, int sequences, int most, int64_t longest
     const int64_t rows = (int64_t)most * group;
     if (window > 0 && (int64_t)window + sinks + most < longest) longest = (int64_t)window + sinks + most;     // keys that a tile can see
     const int64_t groups = (longest + kKvGroup - 1) / kKvGroup;
-    int64_t tiles;
+    int64_t base;                    // workgroups of one share
     auto cut = [&](int tile_rows) {
         p.tile_rows = tile_rows;
         p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
-        tiles = (int64_t)sequences * p.tiles;
+        int64_t tiles = (int64_t)sequences * p.tiles;
         p.slots = tiles * heads * tile_rows;
         // packed rows bound the tiles of all sequences together: whole ones, and one for what is left of each
-        if (tile_rows > 16 && all_rows * group / tile_rows + sequences < tiles) tiles = all_rows * group / tile_rows + sequences;
+        if (p.tiles > 1 && all_rows * group / tile_rows + sequences < tiles) tiles = all_rows * group / tile_rows + sequences;
+        base = tiles * heads;
+        int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
+        if (splits > groups / kv_min_share(tile_rows)) splits = groups / kv_min_share(tile_rows);
+        if (tile_rows > 16 && splits < 4) splits = 1;
+        p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
+        return base * p.splits;
     };
-    cut(kKvTileRows);
-    const int64_t large = tiles * heads * (groups < 32 ? 1 : groups / 16);
-    if (rows <= 64 || (dtype == VAMD_F32 ? dim > 128 || large <= 512 : large <= 128)) cut(16);
-    const int64_t base = tiles * heads;
-    const int least = kv_min_share(p.tile_rows);
-    int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
-    if (splits > groups / least) splits = groups / least;
-    p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
+    const bool large = rows > 64 && !(dtype == VAMD_F32 && dim > 128);
+    if (!large || (cut(128) < (dim > 128 ? 256 : 512) && cut(64) <= 256)) cut(16);
     p.grid = base * p.splits;
     return p;
 }
@@ -883,9 +895,10 @@ template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, 
     return 0;
 }
 
-template <typename T, int FMT, int DT> static int kv_launch_tile_of(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
+template <typename T, int FMT, int DT, int KW> static int kv_launch_tile_of(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
     constexpr int LDS = 2 * 2 * DT * 4 * 64 * 16;
-    auto kernel = kv_attend_tile_kernel<T, FMT, DT, 1>;
+    static_assert(KW == 1 || LDS >= 2 * (DT * 16 + 2) * 64 * 4, "the waves' results pass through the buffers");
+    auto kernel = kv_attend_tile_kernel<T, FMT, DT, KW>;
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return fail((int)e, "vamd_kv_attend: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
@@ -894,18 +907,18 @@ template <typename T, int FMT, int DT> static int kv_launch_tile_of(const KvAtte
     VAMD_LAUNCH_OK("kv_attend_tile");
     return 0;
 }
-template <typename T, int FMT> static int kv_launch_tile(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
+template <typename T, int FMT, int KW> static int kv_launch_tile(const KvAttendArgs& a, int64_t grid, hipStream_t st) {
     switch ((a.D + 31) / 32) {
-        case 1: return kv_launch_tile_of<T, FMT, 1>(a, grid, st);
-        case 2: return kv_launch_tile_of<T, FMT, 2>(a, grid, st);
-        case 3: return kv_launch_tile_of<T, FMT, 3>(a, grid, st);
-        case 4: return kv_launch_tile_of<T, FMT, 4>(a, grid, st);
+        case 1: return kv_launch_tile_of<T, FMT, 1, KW>(a, grid, st);
+        case 2: return kv_launch_tile_of<T, FMT, 2, KW>(a, grid, st);
+        case 3: return kv_launch_tile_of<T, FMT, 3, KW>(a, grid, st);
+        case 4: return kv_launch_tile_of<T, FMT, 4, KW>(a, grid, st);
     }
     if constexpr (sizeof(T) == 2) {
         switch ((a.D + 31) / 32) {
             case 5:
-            case 6: return kv_launch_tile_of<T, FMT, 6>(a, grid, st);
-            default: return kv_launch_tile_of<T, FMT, 8>(a, grid, st);
+            case 6: return kv_launch_tile_of<T, FMT, 6, KW>(a, grid, st);
+            default: return kv_launch_tile_of<T, FMT, 8, KW>(a, grid, st);
         }
     }
     return fail(VAMD_EUNSUPPORTED, "vamd_kv_attend: no kernel for %d features in float32", a.D);
@@ -1004,6 +1017,7 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     a.sinks = sinks;
     a.causal = causal;
     a.tiles = plan.tiles;
+    a.all_tiles = (int)(plan.grid / plan.splits / heads);
     a.tile_rows = plan.tile_rows;
     a.splits = plan.splits;
     const int n = 16 / size;
@@ -1013,7 +1027,9 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     auto launch = [&](auto t, auto f) {
         using T = decltype(t);
         constexpr int FMT = decltype(f)::value;
-        return plan.tile_rows == 16 ? kv_launch_rows<T, FMT>(a, grid, st) : kv_launch_tile<T, FMT>(a, grid, st);
+        return plan.tile_rows == 16   ? kv_launch_rows<T, FMT>(a, grid, st)
+               : plan.tile_rows == 64 ? kv_launch_tile<T, FMT, 2>(a, grid, st)
+                                      : kv_launch_tile<T, FMT, 1>(a, grid, st);
     };
     const std::integral_constant<int, VAMD_KV_E4M3> e4m3;
     const std::integral_constant<int, VAMD_KV_INT8> int8;
