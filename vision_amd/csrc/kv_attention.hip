@@ -130,8 +130,10 @@ __device__ __forceinline__ kv_u32x4 kv_as_loaded(kv_u32x4 w) {
     return w;
 }
 
-// C: 64-feature chunks of a head (the last one may be partly empty).
-template <typename T, int FMT, int C>
+// C: 64-feature chunks of a head (the last one may be partly empty).  ONCE: one tile of rows, so that every code is read once, past the
+// caches' replacement (256 sequences up to 2000: 117 -> 106 us, 64 up to 4096 64 -> 60); with more tiles the others find them there
+// (two tiles: 67 us, 71 past it).
+template <typename T, int FMT, int C, bool ONCE>
 __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(const KvAttendArgs a) {
     constexpr int N = sizeof(T) == 4 ? 3 : 1;                            // bf16 pieces of a query or probability
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -145,7 +147,10 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     const uint32_t tiles = (uint32_t)a.all_tiles;
     const int split = (int)(id / tiles);
     int tile = (int)(id % tiles), b;
-    if (!kv_whose_tile(a, lane, tile, b)) return;
+    if (ONCE) {
+        b = tile;
+        tile = 0;
+    } else if (!kv_whose_tile(a, lane, tile, b)) return;
     const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * 16;
 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
@@ -202,6 +207,7 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
         const int in_block = group_of(x) & ((1 << (a.block_shift - 6)) - 1);
         return a.codes[kv] + ((at_of(page) << a.block_shift) + in_block * kKvGroup) * a.D;
     };
+    auto load = [](const uint8_t* p) { return ONCE ? __builtin_nontemporal_load((const kv_u32x4*)p) : *(const kv_u32x4*)p; };
     kv_u32x4 kc[4 * C], vc[4 * C];
     float ks = 0.f, vs = 0.f;
     // in a last chunk that the head does not fill, lanes without a slab read the chunk's first one: their queries are zero
@@ -212,14 +218,14 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int c = 0; c < C; ++c) kc[t * C + c] = *(const kv_u32x4*)(p + (t * S + c * 4) * 256 + (c < C - 1 ? k_lane : k_lane_last));
+            for (int c = 0; c < C; ++c) kc[t * C + c] = load(p + (t * S + c * 4) * 256 + (c < C - 1 ? k_lane : k_lane_last));
     };
     auto load_v = [&](int page, int x) {
         const uint8_t* p = bytes_of(1, page, x);
         vs = a.scales[1][at_of(page)];
 #pragma unroll
         for (int s = 0; s < 4 * C; ++s)
-            if (s < S) vc[s] = *(const kv_u32x4*)(p + s * 1024 + k_lane);
+            if (s < S) vc[s] = load(p + s * 1024 + k_lane);
     };
     int x = begin + wave;
     int page = page_of(x), next = page_of(x + 4);
@@ -897,7 +903,10 @@ template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, 
     const int C = (a.D + 63) / 64;
     const size_t lds = (size_t)(2 * 64 * C * 16 + 2 * 64 * 2) * 4;
 #define KV_ROWS(C_)                                                                                                              \
-    case C_: hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_>), dim3((unsigned)grid), dim3(256), lds, st, a); break
+    case C_:                                                                                                                     \
+        if (a.tiles == 1) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, true>), dim3((unsigned)grid), dim3(256), lds, st, a);      \
+        else hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, false>), dim3((unsigned)grid), dim3(256), lds, st, a);        \
+        break
     switch (C) {
         KV_ROWS(1);
         KV_ROWS(2);

@@ -8,7 +8,7 @@
 //      32 bits and one rounding to the code: e4m3 codes only lose bits that fall below the smallest code, int8 codes round again;
 //   3. the rows as codes, from registers where a workgroup can hold them, else read again (from L2): x * 2^-e is exact, the code's
 //      rounding (to nearest, ties to even) is the only one.
-// Bound by memory: 16000 tokens of 8 heads and 128 features (int8, blocks of 128) 28 us written, 21 read back, 3.6 and 4.8 TB/s.  A block belongs to one sequence while it is written: no two
+// Bound by memory: 16000 tokens of 8 heads and 128 features (int8, blocks of 128) 27 us written, 21 read back, 3.8 and 4.8 TB/s.  A block belongs to one sequence while it is written: no two
 // workgroups of a call write the same bytes, nothing is added atomically, the result does not depend on any order.
 #include "kv_layout.h"
 
@@ -61,6 +61,21 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void kv_store8(T*
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = from_f<T>(v[e]);
     }
+}
+
+// Transposes the 4 x 4 dwords of four neighbouring lanes: lane j (0..3) gives r[i] to lane i and gets theirs in order.
+__device__ __forceinline__ void kv_transpose_quad(kv_u32x4& r, int j) {
+    auto trade = [&](int a, int b, bool upper, auto swap) {
+        const uint32_t got = swap(upper ? r[a] : r[b]);
+        r[a] = upper ? got : r[a];
+        r[b] = upper ? r[b] : got;
+    };
+    auto by1 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true); };      // lanes 1 0 3 2
+    auto by2 = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true); };      // lanes 2 3 0 1
+    trade(0, 1, j & 1, by1);
+    trade(2, 3, j & 1, by1);
+    trade(0, 2, j & 2, by2);
+    trade(1, 3, j & 2, by2);
 }
 
 template <int FMT> __device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, float ratio) {
@@ -199,8 +214,23 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     auto quad_at = [&](int g, int p, int gg, int tt) {
         return codes + (int64_t)g * kKvGroup * D + (((p >> 1) * 4 + gg) * 16 + (p & 1) * 8) * 16 + tt * 4;
     };
-    // stores the fresh tokens of a quad (t ..): whole dwords, or their bytes beside others that stay
+    // stores the fresh tokens of a quad (t ..): in a group that is fresh throughout the four lanes of the same features (tiles 0 .. 3) trade
+    // dwords, so that each stores the 16 bytes of two features (with 4-byte stores 16 bytes apart 16000 tokens took 28 us, so 27);
+    // else whole dwords, or their bytes beside others that stay
     auto put_quad = [&](uint8_t* to, const float (&v)[4][8], int t) {
+        const int group = t & ~(kKvGroup - 1), tt = (t >> 4) & 3;
+        if (group >= lo && group + kKvGroup <= hi) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = encode_quad(v, e);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                kv_u32x4 r = {w[half * 4], w[half * 4 + 1], w[half * 4 + 2], w[half * 4 + 3]};
+                kv_transpose_quad(r, tt);
+                *(kv_u32x4*)(to - tt * 4 + (half * 4 + tt) * 16) = r;
+            }
+            return;
+        }
         const bool all = t >= lo && t + 4 <= hi;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -436,8 +466,8 @@ extern "C" int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, co
     // One wave where a block gets at most 4 tokens (a decoding step: no barrier, more blocks a CU), else four.
     const int threads = most <= 4 ? 64 : 256;
     // What four waves hold in registers: blocks up to 16384 elements (64 or 128 tokens of 128 features) with HOLD 2, up to 32768 with 4
-    // (116 and 180 registers; beyond that the rows are read twice).  16000 tokens of 8 heads, 128 features, written and read back: blocks of
-    // 128 tokens 55 us with 2, 66 with 4, 67 read twice; of 256 tokens 60 with 4, 71 read twice.
+    // (beyond that the rows are read twice).  16000 tokens of 8 heads, 128 features, written and read back: blocks of 128 tokens 55 us with
+    // 2, 66 with 4, 67 read twice; of 256 tokens 60 with 4, 71 read twice.
     if (block * dim <= 16384 || threads == 64) VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 2>););
     else VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 4>););
     VAMD_LAUNCH_OK("kv_append");
