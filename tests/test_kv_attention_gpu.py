@@ -107,6 +107,8 @@ def test_window_and_sinks(window, sinks, dtype):
     q = rnd((sum(counts), 6, 64), dtype, 49)
     out = c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), most=max(counts), window=window, sinks=sinks)
     compare(out, q, k, v, off, lengths, counts, 0.125, dtype, window=window, sinks=sinks)
+    if sinks == 2 ** 31 - 1:
+        assert torch.equal(out, c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), most=max(counts), window=window, sinks=2 ** 32 + 1))
     one = c.attend(q[:5], table, i32(lengths), window=window, sinks=sinks)
     compare(one, q[:5], k, v, off, lengths, [1] * 5, 0.125, dtype, window=window, sinks=sinks)
 

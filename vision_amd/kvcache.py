@@ -27,6 +27,7 @@ from . import _lib
 from ._lib import call_on, lib, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_INT_MAX = 2 ** 31 - 1
 _FORMATS = {"e4m3": _lib.KV_E4M3, "int8": _lib.KV_INT8}
 
 
@@ -150,6 +151,7 @@ class KVCache:
         q = self._rows("q", q, heads)
         if window < 0 or sinks < 0 or (window and not causal):
             raise ValueError(f"window {window}, sinks {sinks}: not negative, and a window needs causal queries")
+        window, sinks = min(int(window), _INT_MAX), min(int(sinks), _INT_MAX)
         if out is not None:
             self._written("out", out, q.shape)
             if out.dtype != q.dtype:
