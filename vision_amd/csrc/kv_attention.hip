@@ -7,7 +7,8 @@
 // in one pass over the cache with the running maximum m, sum and output (fp32, exponents in base 2).
 //
 // kv_attend_rows_kernel: few queries (a decoding step).  A tile is up to 16 rows (query tokens x heads of one key head), so that
-// every code of the cache is read once for all heads that share it; bound by reading the cache.  Each of a workgroup's four
+// every code of the cache is read once for all heads that share it; bound by reading the cache (64 sequences of up to 4096, 8 key heads
+// of 128 features: 56 us, 4.7 TB/s).  Each of a workgroup's four
 // waves takes every fourth group of 64 tokens of its share of the keys; codes go straight from global memory into MFMA
 // operand order (16 bytes a lane, 1 KB a wave and load) and become bf16 in registers: code values are exact there.  With the keys as the
 // rows of the first product a lane holds 16 scores of ONE query, and exactly the slots that the second product wants as its
@@ -131,7 +132,7 @@ __device__ __forceinline__ kv_u32x4 kv_as_loaded(kv_u32x4 w) {
 }
 
 // C: 64-feature chunks of a head (the last one may be partly empty).  ONCE: one tile of rows, so that every code is read once, past the
-// caches' replacement (256 sequences up to 2000: 117 -> 106 us, 64 up to 4096 64 -> 60); with more tiles the others find them there
+// caches' replacement (256 sequences up to 2000: 117 -> 103 us, 64 up to 4096 64 -> 56); with more tiles the others find them there
 // (two tiles: 67 us, 71 past it).
 template <typename T, int FMT, int C, bool ONCE>
 __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(const KvAttendArgs a) {
@@ -425,8 +426,8 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 // scale goes into the exponent.
 //
 // Bound by the matrix cores, the exponentials and the LDS reads about alike (an operand is read once for 32 queries, 128 bytes a
-// clock): 30000 keys before 2048 queries of 32 heads, 128 features, 936 TFLOP/s; prompts of 4096 and 925 tokens behind
-// 1000 780, where causal tiles of unlike length leave some of the chip idle; a plain bf16 product of 8192^3 reaches 1234.
+// clock): 30000 keys before 2048 queries of 32 heads, 128 features, 938 TFLOP/s; prompts of 4096 and 925 tokens behind
+// 1000 760 to 840, where causal tiles of unlike length leave some of the chip idle; a plain bf16 product of 8192^3 reaches 1234.
 //
 // DT: tiles of 32 features (the last may be half empty).
 __device__ __forceinline__ float kv_over_halves_max(float v) {               // over the two lanes that hold one query's keys
@@ -865,8 +866,9 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
 // queries (32) 14 / 17 / 18.  float32 (three products): up to 2 x 2000 queries 202 / 218 / 163, up to 4 x 200 30 / 39 / 51.
 //
 // Then shares of the keys, until 512 workgroups have work.  Tiles of 16: no share less than 8 groups of 64 tokens.  One token of
-// 64 sequences of up to 4096 (8 key heads, 128 features): 61 us with 256 or 512, 70 with 768 and 68 with 1024 workgroups; of
-// one sequence of 131071: 40, 42, 44 and 45 us.  Large tiles, whose partial results are many: only from 4 shares of 16 groups on
+// 64 sequences of up to 4096 (8 key heads, 128 features): 56 us with 256 or 512, 60 with 768 or 1024 workgroups; of
+// one sequence of 131071: 37, 38, 41 and 42 us; 8 queries of 16 sequences of up to 8000 (two tiles): 80, 67, 57 and 62; 30
+// queries of 16 sequences behind 1000: 26, 26, 47 and 47.  Large tiles, whose partial results are many: only from 4 shares of 16 groups on
 // (2048 queries as two shares 140 us, as one 71; 64 queries behind 60000 keys as 32 shares 104).
 struct KvPlan {
     int tile_rows, tiles, splits;    // tiles of a sequence of `most` rows
