@@ -132,6 +132,19 @@ def test_long_contexts_split_and_joined(format, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
+def test_many_short_sequences_without_most(dtype):
+    """Rows of unlike number, none known to the host: few tiles, split along the keys and joined."""
+    counts = [1, 0, 2, 9, 1, 1, 5, 0, 3] * 9
+    lengths = [(700 * i) % 4001 + 9 for i in range(len(counts))]
+    c, table, k, v, off = filled(lengths, 1, 64, 64, "e4m3", 75)
+    q = rnd((sum(counts), 6, 64), dtype, 79)
+    assert lib.vamd_kv_attend_workspace(sum(counts), len(counts), sum(counts), table.shape[1] * 64, 1, 6, 64, 0, 0, _lib.BF16) > 0
+    for window in (0, 1500):
+        out = c.attend(q, table, i32(lengths), offsets=i32(offsets_of(counts)), window=window, sinks=5)
+        compare(out, q, k, v, off, lengths, counts, 0.125, dtype, **(dict(window=window, sinks=5) if window else {}))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
 def test_many_queries(dtype):
     """Prompts of many tiles, behind an earlier context, windowed or not."""
     lengths, counts = [700, 1100], [700, 600]

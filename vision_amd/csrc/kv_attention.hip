@@ -35,7 +35,7 @@ struct KvAttendArgs {
     const int32_t* lengths;
     const int32_t* offsets;
     int64_t rows;
-    float* part;                 // [tile rows][splits][D] outputs, then [tile rows][splits][2] maximum and sum
+    float* part;                 // [tiles of all sequences][heads][tile rows][splits][D] outputs, then [..][splits][2] maximum and sum
     float* part_ml;
     float scale2;                // scale * log2(e)
     int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, all_tiles, tile_rows, splits, q_aligned, o_aligned;
@@ -66,6 +66,8 @@ __device__ __forceinline__ int kv_share(int count, int splits, int tile_rows) {
     const int per = (count + splits - 1) / splits, least = kv_min_share(tile_rows);
     return per < least ? least : per;
 }
+// Rows of a tile that can be there at all.
+__host__ __device__ constexpr int kv_tile_fill(int tiles, int tile_rows, int most, int group) { return tiles > 1 ? tile_rows : most * group; }
 __device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
     const int64_t room = (int64_t)a.width << a.block_shift;
     int n = a.lengths[b];
@@ -148,11 +150,11 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     const uint32_t tiles = (uint32_t)a.all_tiles;
     const int split = (int)(id / tiles);
     int tile = (int)(id % tiles), b;
+    const int64_t slot = ((int64_t)tile * a.heads + h) * 16;
     if (ONCE) {
         b = tile;
         tile = 0;
     } else if (!kv_whose_tile(a, lane, tile, b)) return;
-    const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * 16;
 
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     if (tile * 16 >= rows.count * a.group) return;
@@ -457,12 +459,12 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
     id /= (uint32_t)a.heads;
     const int split = (int)(id % (uint32_t)a.splits);
     int tile = (int)(id / (uint32_t)a.splits), b;
+    const int64_t slot = ((int64_t)tile * a.heads + h) * a.tile_rows;
     if (!kv_whose_tile(a, lane, tile, b)) return;
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int all_rows = rows.count * a.group;
     tile = (all_rows + a.tile_rows - 1) / a.tile_rows - 1 - tile;
     if (tile < 0) return;
-    const int64_t slot = (((int64_t)b * a.heads + h) * a.tiles + tile) * a.tile_rows;
     const int first_row = tile * a.tile_rows;
     const int length = kv_length(a, b), shift = length - (int)rows.all;
     const int last_row = first_row + a.tile_rows - 1 < all_rows ? first_row + a.tile_rows - 1 : all_rows - 1;
@@ -798,15 +800,19 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     __shared__ __attribute__((aligned(16))) float box[kKvJoin * 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint32_t id = blockIdx.x;
-    const uint32_t per_head = (uint32_t)a.most * a.group;
-    const int row = (int)(id % per_head);
-    id /= per_head;
-    const int64_t slot = (int64_t)id * a.tiles * a.tile_rows + row;
-    const int h = (int)(id % (uint32_t)a.heads), b = (int)(id / (uint32_t)a.heads);
+    const uint32_t per_tile = (uint32_t)kv_tile_fill(a.tiles, a.tile_rows, a.most, a.group);
+    int row = (int)(id % per_tile);
+    id /= per_tile;
+    const int64_t slot = (int64_t)id * a.tile_rows + row;
+    const int h = (int)(id % (uint32_t)a.heads);
+    int tile = (int)(id / (uint32_t)a.heads), b;
+    if (!kv_whose_tile(a, lane, tile, b)) return;
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
+    if (a.tile_rows > 16) tile = (rows.count * a.group + a.tile_rows - 1) / a.tile_rows - 1 - tile;      // the tile kernel's order
+    row += tile * a.tile_rows;
     const int tok = row / a.group;
-    if (tok >= rows.count) return;
-    const int length = kv_length(a, b), shift = length - (int)rows.all, r0 = row / a.tile_rows * a.tile_rows;
+    if (tile < 0 || tok >= rows.count) return;
+    const int length = kv_length(a, b), shift = length - (int)rows.all, r0 = tile * a.tile_rows;
     const int r1 = r0 + a.tile_rows < rows.count * a.group ? r0 + a.tile_rows - 1 : rows.count * a.group - 1;
     const KvRange range = kv_range(a, length, a.causal ? shift + r0 / a.group : length - 1, a.causal ? shift + r1 / a.group : length - 1);
     const int per = kv_share(range.count, a.splits, a.tile_rows);
@@ -885,10 +891,10 @@ static KvPlan kv_plan(int64_t all_rows, int sequences, int most, int64_t longest
         p.tile_rows = tile_rows;
         p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
         int64_t tiles = (int64_t)sequences * p.tiles;
-        p.slots = tiles * heads * tile_rows;
         // packed rows bound the tiles of all sequences together: whole ones, and one for what is left of each
         if (p.tiles > 1 && all_rows * group / tile_rows + sequences < tiles) tiles = all_rows * group / tile_rows + sequences;
         base = tiles * heads;
+        p.slots = base * tile_rows;
         int64_t splits = base > 0 ? (512 + base - 1) / base : 1;
         if (splits > groups / kv_min_share(tile_rows)) splits = groups / kv_min_share(tile_rows);
         if (tile_rows > 16 && splits < 4) splits = 1;
@@ -952,7 +958,7 @@ template <typename T, int FMT, int KW> static int kv_launch_tile(const KvAttendA
 // One wave per row, four or sixteen: so many that a lane reads about four shares.  32 rows of 256 shares: 12 us with four waves, 5.8 with
 // sixteen; 512 rows of 4 shares (128 features): 18 us with sixteen waves, 4 with one.
 template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream_t st) {
-    const unsigned grid = (unsigned)((int64_t)a.sequences * a.heads * a.most * a.group);
+    const unsigned grid = (unsigned)((int64_t)a.all_tiles * a.heads * kv_tile_fill(a.tiles, a.tile_rows, a.most, a.group));
     const int lanes = a.splits * (a.D / 4) / 4;
     if (lanes <= 64) hipLaunchKernelGGL((kv_join_kernel<T, 64>), dim3(grid), dim3(64), 0, st, a);
     else if (lanes <= 256) hipLaunchKernelGGL((kv_join_kernel<T, 256>), dim3(grid), dim3(256), 0, st, a);
@@ -994,7 +1000,8 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE(window >= 0 && sinks >= 0 && (causal || window == 0), "vamd_kv_attend: window %d, sinks %d (not negative; a window "
                  "needs causal queries)", window, sinks);
     VAMD_REQUIRE((int64_t)width * block <= 0x7fffffc0, "vamd_kv_attend: %d blocks of %d tokens are too many for a sequence", width, block);
-    VAMD_REQUIRE((int64_t)most * group <= 0x7fffffc0 && rows <= 0x7fffffff, "vamd_kv_attend: %d of %lld rows of %d heads are too many for a sequence",
+    // (64 sequences' tiles are counted at once)
+    VAMD_REQUIRE((int64_t)most * group <= 1 << 28 && rows <= 0x7fffffff, "vamd_kv_attend: %d of %lld rows of %d heads are too many for a sequence",
                  most, (long long)rows, group);
     VAMD_REQUIRE(offsets || rows == (int64_t)sequences * most, "vamd_kv_attend: %lld rows are not %d for each of %d sequences",
                  (long long)rows, most, sequences);
@@ -1009,7 +1016,7 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                  "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     const int64_t grid = plan.grid;
-    VAMD_REQUIRE(grid <= 0x7fffffff && (plan.splits == 1 || plan.slots <= 0x7fffffff), "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
+    VAMD_REQUIRE(grid <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
                  sequences, most);
     KvAttendArgs a = {};
     a.q = q;
