@@ -526,7 +526,8 @@ enum { VAMD_KV_E4M3 = 0, VAMD_KV_INT8 = 1 };
 /* Writes rows k, v [rows][heads][dim] at positions start[b], start[b]+1, ... of each sequence.  A block whose first token is
  * written starts anew; otherwise its scale never shrinks, and its codes are moved (rounded once more) when it grows.  A block
  * that is given an infinity or a NaN reads as NaN until it starts anew.  Rows that fall into a hole, behind `width` blocks or before
- * position 0 (start < 0) are dropped.  A block being written belongs to one sequence of the call. */
+ * position 0 (start < 0) are dropped.  A block being written belongs to one sequence of the call, and
+ * once to that. */
 int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
                    void* codes_k, void* codes_v, float* scales_k, float* scales_v, const int32_t* table, int64_t table_stride,
                    const int32_t* start, const int32_t* offsets, int64_t rows, int sequences, int most, int heads, int dim,

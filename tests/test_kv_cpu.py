@@ -1,6 +1,7 @@
 """Rotary positions, the 8-bit cache and attention over it: what can be checked without a GPU.  Refusals of the Python layer and of
 the C entry points (they come before any device work), the frequencies, the index functions of csrc/kv_layout.h compiled for
 the host, and the plain forms the GPU tests compare with."""
+import copy
 import math
 import os
 import random
@@ -181,6 +182,35 @@ def test_attend_refuses_overlapping_out():
         _call("attend", q=x[:2], out=x[1:])
 
 
+def test_overlapping_tells_exactly():
+    import itertools
+    rng, buf, seen = random.Random(1), torch.zeros(400), [0, 0]
+
+    def places(t):
+        return {t.storage_offset() + sum(i * s for i, s in zip(at, t.stride())) for at in itertools.product(*map(range, t.shape))}
+
+    for _ in range(1500):
+        dims = rng.randint(1, 4)
+        strides = [rng.choice((0, 1, 1, 2, 3, 4, 5, 8, 12, 16, 24)) for _ in range(dims)]
+        a, b = (buf.as_strided([rng.randint(1, 4) for _ in range(dims)], strides, rng.randint(0, 60)) for _ in range(2))
+        if rng.random() < 0.5:
+            b = buf.as_strided(b.shape, [rng.choice((0, 1, 2, 3, 7, 16)) for _ in range(dims)], b.storage_offset())
+        want = bool(places(a) & places(b))
+        seen[want] += 1
+        assert _lib.overlapping(a, b) == want == _lib.overlapping(b, a), (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert min(seen) > 300
+    x = torch.zeros(4, 3, 12, 16)                           # queries and keys of one buffer, heads before or behind the tokens
+    for y in (x, x.transpose(1, 2).contiguous().transpose(1, 2)):
+        assert not _lib.overlapping(y[:, :, :8], y[:, :, 8:10]) and _lib.overlapping(y[:, :, :8], y[:, :, 7:9])
+    assert not _lib.overlapping(x, x.clone()) and not _lib.overlapping(x[:0], x)
+
+
+def test_a_copied_cache_is_its_own():
+    c = KVCache(4, 2, 32, device="cpu")
+    d = copy.deepcopy(c)
+    assert not set(c._pool()) & set(d._pool()) and d._pool()[0] == d.codes_k.data_ptr()
+
+
 def io_call(name, **change):
     a = dict(ck=P, cv=P, sk=P, sv=P, table=P, stride=2, start=P, offsets=None, rows=2, sequences=2, most=1, heads=2, dim=32, block=64, width=2,
              blocks=4, format=0, x=P, xt=64, xh=32, y=P, yt=64, yh=32, dtype=0)
@@ -218,7 +248,7 @@ def attend_call(**change):
 @pytest.mark.parametrize("bad", [dict(q=None), dict(o=None), dict(cv=None), dict(sk=None), dict(table=None), dict(lengths=None), dict(q=P + 2),
                                  dict(dim=8), dict(dim=288), dict(block=63), dict(format=-1), dict(dtype=7), dict(window=-1), dict(sinks=-1),
                                  dict(window=2, causal=0), dict(rows=3), dict(heads=0), dict(group=0), dict(width=0), dict(blocks=0),
-                                 dict(width=2 ** 30), dict(most=2 ** 30, group=4, rows=2 ** 31), dict(longest=1 << 20),   # workspace needed, none given
+                                 dict(width=2 ** 30), dict(most=2 ** 30, group=4, rows=2 ** 31), dict(most=2 ** 28 + 1, rows=2 ** 29 + 2), dict(longest=1 << 20),   # workspace needed, none given
                                  dict(longest=1 << 20, work=P + 8, size=1 << 40), dict(lengths=P + 1)])
 def test_attend_entry_refuses(bad):
     assert attend_call(**bad) < 0 and b"vamd_kv_attend" in lib.vamd_last_error()
@@ -227,6 +257,17 @@ def test_attend_entry_refuses(bad):
 def test_attend_entry_with_nothing_to_do():
     assert attend_call(rows=0, most=0) == 0
     assert lib.vamd_kv_attend_workspace(1, 0, 1, 64, 1, 1, 64, 0, 0, 0) == 0
+
+
+def test_attend_workspace_goes_by_the_rows_there_are():
+    """However many rows a sequence might have by `most`: a share per workgroup, of which there are about as many as the chip holds."""
+    for sequences, rows, heads, group, longest in [(255, 510, 1, 8, 1 << 20), (500, 500, 1, 4, 1 << 16), (100, 100, 2, 16, 1 << 18), (3, 900, 1, 1, 1 << 20),
+                                                   (40, 1200, 2, 8, 1 << 20)]:
+        for dim in (64, 256):
+            for most in (1, rows // sequences + 1, rows):
+                tile = lib.vamd_kv_attend_tile(rows, sequences, most, longest, heads, group, dim, 0, 0, _lib.BF16)
+                size = lib.vamd_kv_attend_workspace(rows, sequences, most, longest, heads, group, dim, 0, 0, _lib.BF16)
+                assert size <= 1024 * tile * (dim + 2) * 4, (sequences, rows, most, dim, size)
 
 
 # ---------------------------------------------------------------------------------------------------- index functions, on the host

@@ -125,6 +125,8 @@ def test_in_place(dtype):
         r.apply_(pos, rnd((1, 1, 64), dtype).expand(10, 2, 64))
     with pytest.raises(ValueError, match="same memory"):
         r.apply_(pos, q, q)
+    with pytest.raises(ValueError, match="same memory"):
+        r.apply_(pos, q, qkv[:, 3:5])
     with pytest.raises(RuntimeError, match="gradient"):
         r.apply_(pos, kept.requires_grad_())
     # autograd notices what was overwritten

@@ -220,3 +220,38 @@ def self_overlapping(t):
             return True
         reach += stride * (size - 1)
     return False
+
+
+def overlapping(a, b):
+    """Whether some element of a shares memory with one of b (tensors of one element size): exact, also for pieces of one buffer's rows.
+
+    Elements meet where sum(i * stride of a) - sum(j * stride of b) is the distance of the two; largest strides first, few
+    multiples of each leave a rest that the smaller ones can make up."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or a.numel() == 0 or b.numel() == 0:
+        return False
+    size = a.element_size()
+    ahead = b.data_ptr() - a.data_ptr()
+    u, v = a.stride(), b.stride()
+    if len(u) == len(v) > 2 and u[:-2] == v[:-2] and u[-3] > 0 and ahead % size == 0 and all(s % u[-3] == 0 for s in u[:-3]):
+        # side by side in the rows of one buffer (queries and keys of one projection): told without what follows
+        at = ahead // size % u[-3]
+        if at > (a.shape[-2] - 1) * u[-2] + (a.shape[-1] - 1) * u[-1] and u[-3] - at > (b.shape[-2] - 1) * v[-2] + (b.shape[-1] - 1) * v[-1]:
+            return False
+    ranges = {}                                         # stride -> [least, most] multiple
+    for t, end, sign in ((a, 1, 1), (b, 0, -1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s:
+                ranges.setdefault(s, [0, 0])[end] += sign * (n - 1)
+    low, high = sum(s * r[0] for s, r in ranges.items()), sum(s * r[1] for s, r in ranges.items())
+    if not (low - 1) * size < ahead < (high + 1) * size:
+        return False
+    if ahead % size:
+        return True                                     # (elements may meet in part: not looked at more closely)
+    rests = {ahead // size}
+    for s in sorted(ranges, reverse=True):
+        least, most = ranges[s]
+        low, high = low - s * least, high - s * most    # what the smaller strides can add
+        rests = {rest - d * s for rest in rests for d in range(max(least, -((high - rest) // s)), min(most, (rest - low) // s) + 1)}
+        if len(rests) > 4096:
+            return True
+    return 0 in rests

@@ -24,7 +24,7 @@ The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no g
 import torch
 
 from . import _lib
-from ._lib import call_on, lib, self_overlapping
+from ._lib import call_on, lib, overlapping, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _INT_MAX = 2 ** 31 - 1
@@ -49,10 +49,12 @@ class KVCache:
         self.scales_v = torch.zeros(shape[:2], dtype=torch.float32, device=device)
         self.device = self.codes_k.device
         self._index = self.codes_k.get_device()                  # -1 on the CPU
-        self._pointers = tuple(t.data_ptr() for t in (self.codes_k, self.codes_v, self.scales_k, self.scales_v))
         self._format = _FORMATS[format]
 
     # ---- checks
+
+    def _pool(self):
+        return self.codes_k.data_ptr(), self.codes_v.data_ptr(), self.scales_k.data_ptr(), self.scales_v.data_ptr()
 
     def _rows(self, name, t, heads):
         if t.dtype not in _TYPES:
@@ -106,14 +108,14 @@ class KVCache:
         """Writes rows k, v at positions start[b], start[b]+1, ... of their sequences.  A block whose first token is written starts
         anew (whatever it held behind that is gone); otherwise its scale grows if the rows need it, and its codes move along.  A block
         that gets an infinity or a NaN reads as NaN until it starts anew.  Rows in holes, behind the table's end or of a sequence
-        with start < 0 are dropped.  A block that is written must belong to one sequence of the call."""
+        with start < 0 are dropped.  A block that is written must belong to one sequence of the call, and once to that."""
         k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError(f"k and v differ: {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
         rows = k.shape[0]
         batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
-        call_on(self.device, "vamd_kv_append", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], *self._pointers, *batch, rows, n, most,
+        call_on(self.device, "vamd_kv_append", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], *self._pool(), *batch, rows, n, most,
                 self.kv_heads, self.head_dim, self.block, width, self.blocks, self._format, _TYPES[k.dtype])
 
     def read(self, table, start, rows, offsets=None, most=None, dtype=torch.bfloat16, out=None):
@@ -132,10 +134,11 @@ class KVCache:
                 self._written(name, t, (rows, self.kv_heads, self.head_dim))
             if k.dtype != v.dtype:
                 raise ValueError(f"out: {k.dtype} and {v.dtype}")
-            self._apart("out's two tensors", k, v)
+            if overlapping(k, v):
+                raise ValueError("out's two tensors share memory")
         batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
         ks, vs = k.stride(), v.stride()
-        call_on(self.device, "vamd_kv_read", *self._pointers, *batch, rows, n, most, self.kv_heads, self.head_dim, self.block, width,
+        call_on(self.device, "vamd_kv_read", *self._pool(), *batch, rows, n, most, self.kv_heads, self.head_dim, self.block, width,
                 self.blocks, self._format, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _TYPES[k.dtype])
         return k, v
 
@@ -157,8 +160,8 @@ class KVCache:
             if out.dtype != q.dtype:
                 raise ValueError(f"out is {out.dtype}, q {q.dtype}")
             # every row's queries are read before its result is written: the two may be the same memory
-            if q.data_ptr() != out.data_ptr() or q.stride() != out.stride():
-                self._apart("q and out", q, out)
+            if (q.data_ptr() != out.data_ptr() or q.stride() != out.stride()) and overlapping(q, out):
+                raise ValueError("q and out share memory")
         rows = q.shape[0]
         batch, n, width, most = self._batch(table, "lengths", lengths, offsets, rows, most)
         if out is None:
@@ -169,7 +172,7 @@ class KVCache:
         size = lib.vamd_kv_attend_workspace(rows, n, most, longest, self.kv_heads, group, self.head_dim, window, sinks, _TYPES[q.dtype])
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         qs, os = q.stride(), out.stride()
-        call_on(self.device, "vamd_kv_attend", q.data_ptr(), qs[0], qs[1], *self._pointers, *batch, rows, n, most, longest, self.kv_heads,
+        call_on(self.device, "vamd_kv_attend", q.data_ptr(), qs[0], qs[1], *self._pool(), *batch, rows, n, most, longest, self.kv_heads,
                 group, self.head_dim, self.block, width, self.blocks, self._format, self.head_dim ** -0.5 if scale is None else float(scale),
                 bool(causal), window, sinks, out.data_ptr(), os[0], os[1], None if work is None else work.data_ptr(), size, _TYPES[q.dtype])
         return out
@@ -181,18 +184,3 @@ class KVCache:
             raise RuntimeError(f"{name} requires a gradient: the cache passes none (use torch.no_grad())")
         if t.numel() and (t.stride(2) != 1 or self_overlapping(t)):
             raise ValueError(f"{name} with strides {t.stride()} cannot be written: adjacent features, no element twice")
-
-    @staticmethod
-    def _apart(names, a, b):
-        """Two tensors of a call may lie side by side in the rows of one, but not overlap."""
-        if a.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
-            return
-        reach = [1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) for t in (a, b)]
-        ahead = (b.data_ptr() - a.data_ptr()) // a.element_size()
-        if ahead >= reach[0] or -ahead >= reach[1]:
-            return
-        step = a.stride(0)
-        inner = [1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (a, b)]
-        if step == b.stride(0) and step > 0 and ahead % step >= inner[0] and step - ahead % step >= inner[1]:
-            return
-        raise ValueError(f"{names} share memory")

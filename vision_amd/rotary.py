@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._lib import call_on, self_overlapping
+from ._lib import call_on, overlapping, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _PI = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
@@ -217,8 +217,8 @@ class Rotary(nn.Module):
                 raise RuntimeError(f"{name} requires a gradient: apply_ is not differentiable, call the module instead")
             if t.numel() and (t.stride(-1) != 1 or _layout(t) is None or self_overlapping(t)):
                 raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
-        if k is not None and q.numel() and k.numel() and q.data_ptr() == k.data_ptr():
-            raise ValueError("q and k are the same memory")
+        if k is not None and overlapping(q, k):
+            raise ValueError("q and k are the same memory, or share some of it")
         for t in (q, k):
             if t is not None and t.numel() and not t.is_inference():
                 torch.autograd.graph.increment_version(t)
