@@ -270,6 +270,15 @@ def test_attend_workspace_goes_by_the_rows_there_are():
                 assert size <= 1024 * tile * (dim + 2) * 4, (sequences, rows, most, dim, size)
 
 
+def test_attend_tiles_go_by_the_rows_there_are():
+    def tile(rows, sequences, most, heads=8, group=4, dim=128):
+        return lib.vamd_kv_attend_tile(rows, sequences, most, 4096, heads, group, dim, 0, 0, _lib.BF16)
+    for heads, group, dim in [(8, 4, 128), (1, 8, 256), (4, 2, 64)]:         # two queries each, whether that is known or not
+        assert tile(510, 255, 2, heads, group, dim) == tile(510, 255, 510, heads, group, dim) == 16
+    assert tile(5021, 2, 4096) == tile(5021, 2, 5021) == tile(4096 + 63, 64, 4096) == 128       # prompts, with decoding steps beside them
+    assert tile(800, 4, 200) == tile(800, 4, 800) == 64
+
+
 # ---------------------------------------------------------------------------------------------------- index functions, on the host
 
 HOST = r'''
