@@ -866,9 +866,9 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
 // How a call is cut.
 //
 // Tiles of 16 rows of a (sequence, key head), or of 128 or 64 where these are enough to fill the chip, which has room for 512 (for more
-// than 128 features 256) workgroups of them: 128 rows from 512 workgroups on, 64 above 256, and only where a sequence's rows
-// fill half a tile on average (255 sequences of 2 queries behind 1000, `most` given as 510: 109 us in tiles of 16, 164 of 64).  us with 8 key heads of 128 features
-// and groups of 4 (16 / 64 / 128 rows): 2048 queries (512 tiles of 128) 150 / 92 / 75; up to 4 x 1024 behind 8000 keys 355 / 255 / 240; 4096
+// than 128 features 256) workgroups of them: 128 rows from 512 workgroups on, 64 above 256, and only where a sequence has
+// more than 16 rows on average (255 sequences of 2 queries behind 1000, `most` given as 510: 109 us in tiles of 16, 164 of 64).
+// us with 8 key heads of 128 features and groups of 4 (16 / 64 / 128 rows): 2048 queries (512 tiles of 128) 150 / 92 / 75; up to 4 x 1024 behind 8000 keys 355 / 255 / 240; 4096
 // queries of 8 ungrouped heads of 64 features 84 / 71 / 86; 512 queries (128 tiles) 30 / 24 / 28; 16 x 30 behind 1000 (128) 26 / 34 / 41; 100
 // queries (32) 14 / 17 / 18.  float32 (three products): up to 2 x 2000 queries 202 / 218 / 163, up to 4 x 200 30 / 39 / 51.
 //
@@ -900,9 +900,9 @@ static KvPlan kv_plan(int64_t all_rows, int sequences, int most, int64_t longest
         if (splits > groups / kv_min_share(tile_rows)) splits = groups / kv_min_share(tile_rows);
         if (tile_rows > 16 && splits < 4) splits = 1;
         p.splits = splits < 1 ? 1 : splits > kKvMaxSplits ? kKvMaxSplits : (int)splits;
-        return 2 * all_rows * group >= sequences * (int64_t)tile_rows ? base * p.splits : 0;
+        return base * p.splits;
     };
-    const bool large = rows > 64 && !(dtype == VAMD_F32 && dim > 128);
+    const bool large = rows > 64 && all_rows * group > 16 * (int64_t)sequences && !(dtype == VAMD_F32 && dim > 128);
     if (!large || (cut(128) < (dim > 128 ? 256 : 512) && cut(64) <= 256)) cut(16);
     p.grid = base * p.splits;
     return p;
