@@ -363,3 +363,37 @@ def test_plain_cache_moves_codes_when_a_scale_grows():
     assert c.blocks[0][1] == 4.0 and c.read(0, 2, 2).tolist() == [[100.0, 0.0], [300.0, -4.0]]
     c.append(torch.tensor([[1.0, 1.0]], dtype=torch.float64), 0)                  # begins the block anew
     assert c.blocks[0][1] == 2.0 ** -6
+
+
+# ---------------------------------------------------------------------------------------------------- launches
+
+GRID = r'''
+#include "common.h"
+using namespace vamd;
+int main() {
+    const int64_t counts[] = {1, 2, 65535, 65536, kGridFlat - 1, kGridFlat, kGridFlat + 1, 16777215, 16777216, 16777217, 0x40000001, kGridMost};
+    for (int64_t n : counts) {
+        const dim3 g = grid_of(n);
+        if ((uint64_t)g.x * 256 >= 1ull << 32 || g.y > 65535 || g.z != 1) return 1;          // extents in threads, 32 bits each
+        if ((int64_t)g.x * g.y < n || (int64_t)g.x * g.y >= n + kGridRow) return 2;
+        if (g.y > 1 && g.x != kGridRow) return 3;                                             // what block_number() takes a row to be
+    }
+    return 0;
+}
+'''
+
+
+def test_a_launch_holds_all_its_workgroups(tmp_path):
+    src = tmp_path / "grid.hip"
+    src.write_text(GRID)
+    exe = str(tmp_path / "grid")
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-I",
+                    os.path.join(ROOT, "vision_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True)
+    assert subprocess.run([exe]).returncode == 0
+
+
+def test_calls_whose_size_passes_64_bits_are_refused():
+    most = 2 ** 31 - 1
+    assert rotary_call(batch=most, tokens=most, dim=65536, turned=2, q_heads=65536) < 0 and b"too many" in lib.vamd_last_error()
+    for name in ("vamd_kv_append", "vamd_kv_read"):
+        assert io_call(name, sequences=most, most=most, rows=most, offsets=P, heads=65536) < 0 and b"too many" in lib.vamd_last_error()

@@ -63,6 +63,16 @@ static inline int grid_for(int64_t work_items, int block, int max_blocks = 4096)
     return (int)g;
 }
 
+// Launches of any number of workgroups.  HIP counts each extent of a launch in threads with 32 bits and drops the rest without an
+// error (of 4.5e9 threads in x the last 2e8 never ran), so beyond 2^22 workgroups (of up to 1023 threads) they are laid out
+// kGridRow to a row of the grid; the last row's may lie behind `blocks`, and kernels return there.
+constexpr int64_t kGridFlat = 1 << 22, kGridRow = 1 << 16, kGridMost = 0x7fffffff;
+static inline dim3 grid_of(int64_t blocks) {               // blocks: 1 .. kGridMost
+    if (blocks <= kGridFlat) return dim3((unsigned)blocks);
+    return dim3((unsigned)kGridRow, (unsigned)((blocks + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ uint32_t block_number() { return blockIdx.y * (uint32_t)kGridRow + blockIdx.x; }
+
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(bf16_t x) { return (float)x; }
 template <typename T> __device__ __forceinline__ T from_f(float x);

@@ -144,11 +144,12 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
     const int r = lane & 15, g = lane >> 4;
     // Heads vary fastest, then the tiles, shares slowest: workgroups without work (shares that a short sequence does not have) then sit
     // behind each other and not on every second XCD or CU.
-    uint32_t id = blockIdx.x;
+    uint32_t id = block_number();
     const int h = (int)(id % (uint32_t)a.heads);
     id /= (uint32_t)a.heads;
     const uint32_t tiles = (uint32_t)a.all_tiles;
     const int split = (int)(id / tiles);
+    if (split >= a.splits) return;
     int tile = (int)(id % tiles), b;
     const int64_t slot = ((int64_t)tile * a.heads + h) * 16;
     if (ONCE) {
@@ -454,11 +455,12 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
     const int c = lane & 31, hh = lane >> 5, wave_r = wave % ROW_WAVES, kh0 = wave / ROW_WAVES;
     // Heads vary fastest (where they are a multiple of 8 the tiles of one meet in one XCD's L2), then the shares, then the tiles, late
     // ones of a sequence (the longest, where queries are causal) first.
-    uint32_t id = blockIdx.x;
+    uint32_t id = block_number();
     const int h = (int)(id % (uint32_t)a.heads);
     id /= (uint32_t)a.heads;
     const int split = (int)(id % (uint32_t)a.splits);
     int tile = (int)(id / (uint32_t)a.splits), b;
+    if (tile >= a.all_tiles) return;
     const int64_t slot = ((int64_t)tile * a.heads + h) * a.tile_rows;
     if (!kv_whose_tile(a, lane, tile, b)) return;
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
@@ -913,8 +915,8 @@ template <typename T, int FMT> static int kv_launch_rows(const KvAttendArgs& a, 
     const size_t lds = (size_t)(2 * 64 * C * 16 + 2 * 64 * 2) * 4;
 #define KV_ROWS(C_)                                                                                                              \
     case C_:                                                                                                                     \
-        if (a.tiles == 1) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, true>), dim3((unsigned)grid), dim3(256), lds, st, a);      \
-        else hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, false>), dim3((unsigned)grid), dim3(256), lds, st, a);        \
+        if (a.tiles == 1) hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, true>), grid_of(grid), dim3(256), lds, st, a);      \
+        else hipLaunchKernelGGL((kv_attend_rows_kernel<T, FMT, C_, false>), grid_of(grid), dim3(256), lds, st, a);        \
         break
     switch (C) {
         KV_ROWS(1);
@@ -935,7 +937,7 @@ template <typename T, int FMT, int DT, int KW> static int kv_launch_tile_of(cons
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return fail((int)e, "vamd_kv_attend: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kKvTileThreads), LDS, st, a);
+    hipLaunchKernelGGL(kernel, grid_of(grid), dim3(kKvTileThreads), LDS, st, a);
     VAMD_LAUNCH_OK("kv_attend_tile");
     return 0;
 }
@@ -1017,7 +1019,7 @@ extern "C" int vamd_kv_attend(const void* q, int64_t q_token, int64_t q_head, co
     VAMD_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
                  "vamd_kv_attend: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     const int64_t grid = plan.grid;
-    VAMD_REQUIRE(grid <= 0x7fffffff, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
+    VAMD_REQUIRE(grid <= kGridMost, "vamd_kv_attend: %d sequences of up to %d rows are too many for one call",
                  sequences, most);
     KvAttendArgs a = {};
     a.q = q;

@@ -25,7 +25,7 @@ struct KvIoArgs {
     const int32_t* start;        // position of a sequence's first row
     const int32_t* offsets;
     int64_t rows;
-    int heads, D, block, width, blocks, most, touched;
+    int sequences, heads, D, block, width, blocks, most, touched;
 };
 
 template <typename T, bool ALIGNED> __device__ __forceinline__ Vec16<T> kv_load16(const T* p) {
@@ -86,12 +86,13 @@ template <int FMT> __device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, f
 template <typename T, int FMT, bool ALIGNED, int HOLD>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     __shared__ uint32_t tops[4];
-    int64_t id = blockIdx.x;
+    int64_t id = block_number();
     const int h = (int)(id % a.heads);
     id /= a.heads;
     const int kv = (int)(id & 1);
     id >>= 1;
     const int j = (int)(id % a.touched), b = (int)(id / a.touched);
+    if (b >= a.sequences) return;
     const int64_t start = a.start[b];
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int64_t blk = start / a.block + j, base = blk * a.block;
@@ -332,12 +333,13 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
 // Reading back: one workgroup per (sequence, group of 64 tokens, keys or values, head); a code's value is code * scale, exact.
 template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvIoArgs a) {
-    int64_t id = blockIdx.x;
+    int64_t id = block_number();
     const int h = (int)(id % a.heads);
     id /= a.heads;
     const int kv = (int)(id & 1);
     id >>= 1;
     const int j = (int)(id % a.touched), b = (int)(id / a.touched);
+    if (b >= a.sequences) return;
     const int64_t start = a.start[b];
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int64_t base = (start / kKvGroup + j) * kKvGroup;
@@ -408,6 +410,7 @@ static int kv_io_args(KvIoArgs& a, const char* name, const void* codes_k, const 
     a.start = start;
     a.offsets = offsets;
     a.rows = rows;
+    a.sequences = sequences;
     a.heads = heads;
     a.D = dim;
     a.block = block;
@@ -416,7 +419,7 @@ static int kv_io_args(KvIoArgs& a, const char* name, const void* codes_k, const 
     a.most = most;
     a.touched = (int)(((int64_t)most + unit - 2) / unit + 1);    // blocks or groups that `most` rows reach at worst
     grid = (int64_t)sequences * a.touched * 2 * heads;
-    VAMD_REQUIRE(grid <= 0x7fffffff, "%s: %d sequences of up to %d rows and %d heads are too many for one call", name, sequences, most, heads);
+    VAMD_REQUIRE((double)sequences * a.touched * 2 * heads <= kGridMost, "%s: %d sequences of up to %d rows and %d heads are too many for one call", name, sequences, most, heads);
     return 0;
 }
 static bool kv_aligned(const KvIoArgs& a, const void* p, const void* q, int dtype) {
@@ -428,7 +431,7 @@ static bool kv_aligned(const KvIoArgs& a, const void* p, const void* q, int dtyp
 // KERNEL, which names T, F (format) and A (aligned), for this call's format and alignment; T from VAMD_DISPATCH around it
 #define KV_IO_LAUNCH(KERNEL)                                                                                                     \
     do {                                                                                                                         \
-        const dim3 g((unsigned)grid), t(threads);                                                                                \
+        const dim3 g = grid_of(grid), t(threads);                                                                                \
         if (format == VAMD_KV_E4M3) {                                                                                            \
             constexpr int F = VAMD_KV_E4M3;                                                                                      \
             if (aligned) { constexpr bool A = true; hipLaunchKernelGGL((KERNEL), g, t, 0, as_stream(stream), a); }                \

@@ -55,7 +55,7 @@ template <typename T, int V> struct alignas(sizeof(T) * V) RotaryPiece { T v[V];
 template <typename T, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     typedef RotaryPiece<T, V> Piece;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t id = (int64_t)block_number() * 256 + threadIdx.x;
     const int64_t rest = id / a.chunks;
     const int chunk = (int)(id - rest * a.chunks);
     const int64_t at = rest / a.slots;
@@ -145,11 +145,13 @@ template <typename T> static int rotary_launch(RotaryArgs& a, hipStream_t st) {
     const int heads = a.t[0].heads + a.t[1].heads;
     // A lane walks over 8 heads once that still leaves 16 waves to each of the 256 CUs, over fewer before that.
     a.per = 8;
-    while (a.per > 1 && a.batch * a.tokens * a.chunks * ((heads + a.per - 1) / a.per) < 256 * 16 * 64) a.per >>= 1;
+    const double lanes = (double)(a.batch * a.tokens) * a.chunks;      // (of one head; the product with the heads' may pass 64 bits)
+    while (a.per > 1 && lanes * ((heads + a.per - 1) / a.per) < 256 * 16 * 64) a.per >>= 1;
     a.slots = (heads + a.per - 1) / a.per;
+    VAMD_REQUIRE(lanes * a.slots <= 256.0 * kGridMost, "vamd_rotary: %lld tokens of %d heads are too many for one call",
+                 (long long)(a.batch * a.tokens), heads);
     const int64_t blocks = (a.batch * a.tokens * a.chunks * a.slots + 255) / 256;
-    VAMD_REQUIRE(blocks <= 0x7fffffff, "vamd_rotary: %lld tokens of %d heads are too many for one call", (long long)(a.batch * a.tokens), heads);
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid = grid_of(blocks);
     if (V == 8) {
         if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((rotary_kernel<T, 8>), grid, dim3(256), 0, st, a);
     } else if (V == 4) hipLaunchKernelGGL((rotary_kernel<T, 4>), grid, dim3(256), 0, st, a);
