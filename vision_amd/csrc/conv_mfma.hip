@@ -977,8 +977,11 @@ conv_ntw_mfma_kernel(Gather gp, const T* __restrict__ x, const T* __restrict__ w
     // the MFMAs of the previous half run, so the eight lock-stepped waves never wait on LDS with
     // the matrix pipe idle.  One barrier per K-step, in its middle: before it a wave has waited for
     // its own loads of the next stage, after it the first half of that stage may be read.
-    // fp32: one set, each half read right before its MFMAs (four times the MFMAs per fragment hide the latency).  With two sets
-    // next to the statistics' sums the kernel spilled 70 registers, and the compiler lost some of the sums among them.
+    // fp32: one set, each half read right before its MFMAs (four times the MFMAs per fragment hide the latency: a float32 training step
+    // of 64 images at 224 x 224 89.4 ms with either).  With two sets next to the statistics' sums the register allocator had to move the
+    // sums between registers, and where the lanes meet again behind a residual term's `if (valid[i] && piece_ok[p])` it put
+    // those copies in front of the instruction that brings the skipped lanes back: lanes of rows past the tensor lost their sums.
+    // (tests/test_code_object_cpu.py looks for such places in every kernel of the built library.)
     constexpr bool TWO_SETS = sizeof(T) == 2;
     Frag a0[4], b0[NT], a1[4], b1[NT];
     if constexpr (TWO_SETS) read_frags(0, 0, a0, b0);
@@ -1000,7 +1003,8 @@ conv_ntw_mfma_kernel(Gather gp, const T* __restrict__ x, const T* __restrict__ w
             mma(a0, b0);
             if constexpr (!TWO_SETS) read_frags(buf, 1, a1, b1);
             // the stage read next was issued during the previous K-step: only this K-step's
-            // pixel loads may stay in flight; every LDS read issued so far has long returned
+            // pixel loads may stay in flight; every LDS read issued so far is waited for (bf16: issued before the MFMAs, long
+            // returned; fp32: the second half's were issued just now)
 #if VAMD_ABLATE == 1 || VAMD_ABLATE == 3
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #else

@@ -125,7 +125,7 @@ __device__ __forceinline__ void load16_lds(__amdgpu_buffer_rsrc_t r, uint32_t by
 
 // BatchNorm + LeakyReLU of eight bf16 values held as four 32-bit words, in place: round(leaky(fma(x, sc, sh))) per element,
 // bit for bit what scale_shift_act_kernel stores for slopes in [0, 1] (max(z, slope * z) == z > 0 ? z : slope * z there).
-// Packed fp32 multiply-adds and a two-operand conversion: 32 vector instructions per 16-byte piece.  keep = 0 clears the
+// Multiply-adds element by element (packed fp32 instructions are off) and a two-operand conversion.  keep = 0 clears the
 // piece (a padding pixel, whose zeros must survive the affine map), keep = ~0 leaves it.
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
