@@ -20,9 +20,8 @@ PROBE_LIB = os.path.join(OUT_DIR, "libvamd_probe.so")
 SOURCES = ["elementwise.hip", "norm.hip", "conv_direct.hip", "conv_api.hip", "conv_mfma.hip", "conv_wgrad_halo.hip", "conv_thin.hip",
            "conv_thin_mfma.hip", "attention.hip", "vq.hip", "image.hip", "rotary.hip", "kvcache.hip", "kv_attention.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-# Packed fp32 instructions stay off, as a rule of this build: the compiler forms them from ordinary float code, and operators of these
-# cards report wrong results of some of their forms, now and then and without an error.  (This repository holds no example of
-# one; what the rule costs is in csrc/common.h, as_loaded.)
+# Packed fp32 instructions stay off: the compiler forms them from ordinary float code, and some of their forms are not trusted on
+# these cards (a precaution: this repository holds no example of a wrong result; what it costs is in csrc/common.h, as_loaded).
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          "-Wno-unused-variable", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
