@@ -397,3 +397,39 @@ def test_calls_whose_size_passes_64_bits_are_refused():
     assert rotary_call(batch=most, tokens=most, dim=65536, turned=2, q_heads=65536) < 0 and b"too many" in lib.vamd_last_error()
     for name in ("vamd_kv_append", "vamd_kv_read"):
         assert io_call(name, sequences=most, most=most, rows=most, offsets=P, heads=65536) < 0 and b"too many" in lib.vamd_last_error()
+
+
+# ---------------------------------------------------------------------------------------------------- what torch has to know
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Lets calls with CPU tensors pass up to their launch, and collects those instead."""
+    made = []
+    monkeypatch.setattr(KVCache, "__init__", lambda self, *a, _init=KVCache.__init__, **kw: (_init(self, *a, **kw), setattr(self, "_index", 0))[0])
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    for module in ("vision_amd.kvcache", "vision_amd.rotary"):
+        monkeypatch.setattr(module + ".call_on", lambda device, name, *args: made.append((name, args)))
+    return made
+
+
+def test_autograd_notices_what_is_overwritten(launches):
+    """A backward pass that has saved a tensor which is then given as `out` refuses to run."""
+    def saved(shape):
+        w = torch.ones(shape, requires_grad=True)
+        out = torch.ones(shape)
+        return out, (w * out).sum()
+    out, z = saved((2, 6, 32))
+    _call("attend", out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    for i in range(2):
+        out, z = saved((2, 2, 32))
+        other = torch.zeros(2, 2, 32)
+        _call("read", out=(out, other) if i == 0 else (other, out))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    assert [name for name, _ in launches] == ["vamd_kv_attend", "vamd_kv_read", "vamd_kv_read"]
+    with torch.inference_mode():                            # no version to count there
+        _call("attend", out=torch.ones(2, 6, 32))
+    assert len(launches) == 4

@@ -212,6 +212,13 @@ def call_on(device, name, *args):
         check(rc, name)
 
 
+def overwritten(*tensors):
+    """Tells autograd that a kernel writes into these tensors (None: no tensor): a backward pass that has saved one of them refuses to run."""
+    for t in tensors:
+        if t is not None and t.numel() and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def self_overlapping(t):
     """Whether two elements of t may share memory (as those of an expanded tensor do)."""
     reach = 0

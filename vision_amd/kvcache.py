@@ -24,7 +24,7 @@ The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no g
 import torch
 
 from . import _lib
-from ._lib import call_on, lib, overlapping, self_overlapping
+from ._lib import call_on, lib, overlapping, overwritten, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _INT_MAX = 2 ** 31 - 1
@@ -137,6 +137,8 @@ class KVCache:
             if overlapping(k, v):
                 raise ValueError("out's two tensors share memory")
         batch, n, width, most = self._batch(table, "start", start, offsets, rows, most)
+        if out is not None:
+            overwritten(k, v)
         ks, vs = k.stride(), v.stride()
         call_on(self.device, "vamd_kv_read", *self._pool(), *batch, rows, n, most, self.kv_heads, self.head_dim, self.block, width,
                 self.blocks, self._format, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _TYPES[k.dtype])
@@ -166,6 +168,8 @@ class KVCache:
         batch, n, width, most = self._batch(table, "lengths", lengths, offsets, rows, most)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        else:
+            overwritten(out)
         room = width * self.block
         longest = room if longest is None else min(max(int(longest), 0), room)
         group = heads // self.kv_heads

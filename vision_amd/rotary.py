@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._lib import call_on, overlapping, self_overlapping
+from ._lib import call_on, overlapping, overwritten, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _PI = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
@@ -219,9 +219,7 @@ class Rotary(nn.Module):
                 raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
         if k is not None and overlapping(q, k):
             raise ValueError("q and k are the same memory, or share some of it")
-        for t in (q, k):
-            if t is not None and t.numel() and not t.is_inference():
-                torch.autograd.graph.increment_version(t)
+        overwritten(q, k)
         if q.numel() == 0 or (k is not None and k.numel() == 0):
             if k is not None and (q.numel() or k.numel()):
                 self.apply_(positions, q if q.numel() else k)
