@@ -433,3 +433,25 @@ def test_autograd_notices_what_is_overwritten(launches):
     with torch.inference_mode():                            # no version to count there
         _call("attend", out=torch.ones(2, 6, 32))
     assert len(launches) == 4
+
+
+def test_forward_mode_is_passed_on_or_refused(launches):
+    """A dual tensor's tangent is never dropped.  (What Rotary's tangents are: tests/test_rotary_modes_gpu.py.)"""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        def dual(*shape):
+            return forward_ad.make_dual(torch.ones(shape), torch.ones(shape))
+        r, pos = Rotary(32), torch.arange(2)
+        yq, yk = r(pos, torch.ones(2, 4, 32), dual(2, 1, 32))
+        assert forward_ad.unpack_dual(yq).tangent is None and forward_ad.unpack_dual(yk).tangent.shape == yk.shape
+        assert len(launches) == 3                           # two tensors, one tangent
+        for q, k in ((dual(2, 4, 32), None), (torch.ones(2, 4, 32), dual(2, 1, 32))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                r.apply_(pos, q, k)
+        for method, bad in (("append", lambda: dict(k=dual(2, 2, 32))), ("append", lambda: dict(v=dual(2, 2, 32))), ("attend", lambda: dict(q=dual(2, 6, 32))),
+                            ("attend", lambda: dict(out=dual(2, 6, 32))), ("read", lambda: dict(out=(torch.ones(2, 2, 32), dual(2, 2, 32))))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                _call(method, **bad())
+        assert len(launches) == 3
+        _call("attend")
+    assert len(launches) == 4

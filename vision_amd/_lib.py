@@ -10,6 +10,7 @@ import os
 # device memory and streams handed to this library; loading libvision_amd.so first would pull a
 # second copy of the runtime from /opt/rocm into the process.
 import torch  # noqa: F401
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # VAMD_LIB: another build of the same library (side-by-side kernel experiments)
@@ -217,6 +218,11 @@ def overwritten(*tensors):
     for t in tensors:
         if t is not None and t.numel() and not t.is_inference():
             torch.autograd.graph.increment_version(t)
+
+
+def has_tangent(t):
+    """Whether t is a dual number of forward-mode differentiation (whether or not it requires a gradient)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def self_overlapping(t):

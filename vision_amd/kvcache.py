@@ -24,7 +24,7 @@ The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no g
 import torch
 
 from . import _lib
-from ._lib import call_on, lib, overlapping, overwritten, self_overlapping
+from ._lib import call_on, has_tangent, lib, overlapping, overwritten, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _INT_MAX = 2 ** 31 - 1
@@ -64,6 +64,8 @@ class KVCache:
             raise ValueError(f"{name} has shape {tuple(shape)}, not [rows, {heads}, {self.head_dim}]")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: the cache passes none (use torch.no_grad())")
+        if has_tangent(t):
+            raise RuntimeError(f"{name} carries a tangent: the cache passes none")
         if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         return t if t.stride(2) == 1 else t.contiguous()
@@ -186,5 +188,7 @@ class KVCache:
             raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)} on {t.device}, not float32 or bfloat16 {tuple(shape)} on {self.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient: the cache passes none (use torch.no_grad())")
+        if has_tangent(t):
+            raise RuntimeError(f"{name} carries a tangent: the cache passes none")
         if t.numel() and (t.stride(2) != 1 or self_overlapping(t)):
             raise ValueError(f"{name} with strides {t.stride()} cannot be written: adjacent features, no element twice")

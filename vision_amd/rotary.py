@@ -2,7 +2,7 @@
 sequence model over codebook indices has in place of it.
 
     rotary = Rotary(head_dim, rotary_dim, layout="half", base=10000.0, scaling={"type": "yarn", "factor": 4.0, "original": 8192})
-    q, k = rotary(positions, q, k)                 # differentiable; one kernel for both, one for both gradients
+    q, k = rotary(positions, q, k)                 # differentiable (backward, forward mode); one kernel for both, one for both gradients
     rotary.apply_(positions, q, k)                 # in place, without gradients
 
 q, k: [..., heads, head_dim], float32 or bfloat16 on the GPU, any strides with adjacent features (heads may come before tokens
@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._lib import call_on, overlapping, overwritten, self_overlapping
+from ._lib import call_on, has_tangent, overlapping, overwritten, self_overlapping
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _PI = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
@@ -117,6 +117,8 @@ def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, q, k,
 
 
 def _readable(t):
+    if t is not None and t._is_zerotensor():         # zeros that torch keeps without memory (tangents)
+        t = t.clone()
     return t if t is None or (t.stride(-1) == 1 and (t.dim() <= 4 or _layout(t) is not None)) else t.contiguous()
 
 
@@ -139,6 +141,7 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, positions, frequencies, how, q, k):
         ctx.save_for_backward(positions, frequencies)
+        ctx.save_for_forward(positions, frequencies)
         ctx.how = how
         ctx.set_materialize_grads(False)
         return _turned(positions, frequencies, how, q, k)
@@ -154,6 +157,13 @@ class _RotaryFn(torch.autograd.Function):
         # the transpose of a turn is the turn back, with the same amplitude: the same function, differentiable in turn
         turn = _RotaryFn.apply if torch.is_grad_enabled() else _turned
         return (None, None, None) + tuple(turn(*ctx.saved_tensors, (*ctx.how[:3], 1 - ctx.how[3]), gq, gk))
+
+
+    @staticmethod
+    def jvp(ctx, _positions, _frequencies, _how, tq, tk):
+        # linear: a tangent is turned as its tensor is (forward: q and k both have one, or there is no other)
+        turn = _RotaryFn.apply if torch.is_grad_enabled() else _turned
+        return turn(*ctx.saved_tensors, ctx.how, tq, tk)
 
 
 class Rotary(nn.Module):
@@ -201,8 +211,10 @@ class Rotary(nn.Module):
             if q.numel() == 0 and k.numel() == 0:
                 return q.clone(), k.clone()
             return (self(positions, q), k.clone()) if k.numel() == 0 else (q.clone(), self(positions, k))
-        turn = _turned
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        turn, tangent = _turned, has_tangent(q)
+        if k is not None and has_tangent(k) != tangent:      # torch takes no result without a tangent beside one that has it
+            return self(positions, q), self(positions, k)
+        if tangent or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
             turn = _RotaryFn.apply
         yq, yk = turn(positions, frequencies, self._how, q, k)
         return yq if k is None else (yq, yk)
@@ -215,6 +227,8 @@ class Rotary(nn.Module):
                 continue
             if torch.is_grad_enabled() and t.requires_grad:
                 raise RuntimeError(f"{name} requires a gradient: apply_ is not differentiable, call the module instead")
+            if has_tangent(t):
+                raise RuntimeError(f"{name} carries a tangent: apply_ is not differentiable, call the module instead")
             if t.numel() and (t.stride(-1) != 1 or _layout(t) is None or self_overlapping(t)):
                 raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
         if k is not None and overlapping(q, k):
