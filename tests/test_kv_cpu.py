@@ -455,3 +455,44 @@ def test_forward_mode_is_passed_on_or_refused(launches):
         assert len(launches) == 3
         _call("attend")
     assert len(launches) == 4
+
+
+def _every_call():
+    r, pos = Rotary(32), torch.arange(2)
+    yield "forward", lambda q: r(pos, q)
+    yield "apply_", lambda q: r.apply_(pos, q)
+    c, table, start = KVCache(4, 6, 32, device="cpu"), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    yield "append", lambda q: c.append(q, q, table, start)
+    yield "read", lambda q: c.read(table, start, 2, out=(q, torch.zeros(2, 6, 32)))
+    yield "attend", lambda q: c.attend(q, table, start)
+
+
+def _without_a_launch(monkeypatch):
+    """As `launches`, but with call_on's own checks."""
+    monkeypatch.setattr(KVCache, "__init__", lambda self, *a, _init=KVCache.__init__, **kw: (_init(self, *a, **kw), setattr(self, "_index", 0))[0])
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: None, raising=False)
+    made = []
+    monkeypatch.setattr(_lib, "_entries", {name: lambda *args, name=name: made.append(name) or 0 for name in _lib.SIGNATURES})
+    return made
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_calls_are_not_traced_away(monkeypatch):
+    """A recorded program that lacks the launch would return memory that nobody wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    made = _without_a_launch(monkeypatch)
+    q = torch.ones(2, 6, 32)
+    for name, call in _every_call():
+        call(q)
+        assert len(made) == 1, name
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(call, q)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(call)(q)
+        for transform in (lambda: torch.func.jvp(call, (q,), (q,)), lambda: torch.func.vmap(call)(q[None]), lambda: make_fx(call, tracing_mode="fake")(q)):
+            with pytest.raises(Exception):
+                transform()
+        assert made.pop() and not made, name

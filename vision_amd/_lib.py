@@ -198,11 +198,15 @@ def call(name, *args):
     check(getattr(lib, name)(*args), name)
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 _entries = {name: getattr(lib, name) for name in SIGNATURES}
 
 
 def call_on(device, name, *args):
-    """The same on the current stream of `device` (its last argument), whichever device is current."""
+    """The same on the current stream of `device` (its last argument), whichever device is current.  A kernel launched from here is
+    invisible to what records torch's operators, whose program would return memory that nobody writes: refused there."""
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise RuntimeError(f"{name} cannot be recorded by torch.jit.trace or make_fx: call it outside of the traced function")
     index = device.index
     if index == torch.cuda.current_device():
         rc = _entries[name](*args, torch._C._cuda_getCurrentRawStream(index))
