@@ -2,6 +2,7 @@
 the C entry points (they come before any device work), the frequencies, the index functions of csrc/kv_layout.h compiled for
 the host, and the plain forms the GPU tests compare with."""
 import copy
+import ctypes
 import math
 import os
 import random
@@ -496,3 +497,34 @@ def test_calls_are_not_traced_away(monkeypatch):
             with pytest.raises(Exception):
                 transform()
         assert made.pop() and not made, name
+
+
+def negated(*shape):
+    """A view whose sign torch keeps apart from the memory; features adjacent."""
+    t = torch._neg_view(torch.arange(1.0, 1 + math.prod(shape)).view(shape))
+    assert t.is_neg() and t.stride(-1) == 1
+    return t
+
+
+def test_lazily_negated_views(launches):
+    """Read as what they stand for, not as what lies in memory; not written into."""
+    def floats(at, n):
+        return [x for x in (ctypes.c_float * n).from_address(at)]
+    for name, position, call in (("vamd_rotary", 10, lambda: Rotary(32)(torch.arange(2), negated(2, 6, 32))),
+                                 ("vamd_kv_append", 0, lambda: _call("append", k=negated(2, 2, 32))),
+                                 ("vamd_kv_append", 3, lambda: _call("append", v=negated(2, 2, 32))),
+                                 ("vamd_kv_attend", 0, lambda: _call("attend", q=negated(2, 6, 32)))):
+        launches.clear()
+        hold = []
+        # the launch is where the pointer is valid
+        def look(device, entry, *args):
+            hold.append((entry, floats(args[position], 3)))
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr("vision_amd.kvcache.call_on", look)
+            m.setattr("vision_amd.rotary.call_on", look)
+            call()
+        assert hold == [(name, [-1.0, -2.0, -3.0])]
+    for call in (lambda: Rotary(32).apply_(torch.arange(2), negated(2, 6, 32)), lambda: _call("attend", out=negated(2, 6, 32)),
+                 lambda: _call("read", out=(negated(2, 2, 32), torch.zeros(2, 2, 32)))):
+        with pytest.raises(ValueError, match="lazy sign"):
+            call()

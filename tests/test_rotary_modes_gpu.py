@@ -70,3 +70,38 @@ def test_tangents_against_differences_and_with_a_gradient():
         t = forward_ad.unpack_dual(r(pos, forward_ad.make_dual(q.detach(), d))).tangent
         gd, = torch.autograd.grad((t * w).sum(), d)
     assert torch.equal(gd, g)
+
+
+def test_lazily_negated_queries_and_gradients():
+    r, pos = Rotary(16, device=DEV), torch.arange(4, device=DEV)
+    z = torch.complex(rnd((4, 2, 16), 1), rnd((4, 2, 16), 2))
+    q = z.conj().imag                                        # strides of 2, and the sign apart
+    assert q.is_neg() and torch.equal(r(pos, q), r(pos, -z.imag.contiguous()))
+    x = rnd((4, 2, 16), 3).requires_grad_()
+    g = torch._neg_view(rnd((4, 2, 16), 4))
+    got, = torch.autograd.grad(r(pos, x), x, g)
+    want, = torch.autograd.grad(r(pos, x), x, g.resolve_neg())
+    assert torch.equal(got, want)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_under_torch_compile():
+    """The calls stay calls: what surrounds them may be compiled, the results are the eager ones."""
+    from vision_amd.kvcache import KVCache
+    r, pos = Rotary(64, device=DEV), torch.arange(6, device=DEV)
+    c, table = KVCache(2, 2, 64, device=DEV), torch.tensor([[0, 1]], dtype=torch.int32, device=DEV)
+    start, lengths = torch.zeros(1, dtype=torch.int32, device=DEV), torch.full((1,), 6, dtype=torch.int32, device=DEV)
+
+    def step(q, k, v):
+        q, k = r(pos, q * 2, k)
+        c.append(k, v, table, start)
+        return c.attend(q, table, lengths) + 1
+
+    q, k, v = rnd((6, 4, 64), 1), rnd((6, 2, 64), 2), rnd((6, 2, 64), 3)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(step, backend="eager")(q, k, v), step(q, k, v))
+    x = q.clone().requires_grad_()
+    turn = torch.compile(lambda x: (r(pos, x * 2) ** 2).sum(), backend="eager")
+    got, = torch.autograd.grad(turn(x), x)
+    want, = torch.autograd.grad((r(pos, x * 2) ** 2).sum(), x)
+    assert torch.equal(got, want)

@@ -68,6 +68,7 @@ class KVCache:
             raise RuntimeError(f"{name} carries a tangent: the cache passes none")
         if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+        t = t.resolve_neg()                              # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
         return t if t.stride(2) == 1 else t.contiguous()
 
     def _numbers(self, name, t, size):
@@ -190,5 +191,6 @@ class KVCache:
             raise RuntimeError(f"{name} requires a gradient: the cache passes none (use torch.no_grad())")
         if has_tangent(t):
             raise RuntimeError(f"{name} carries a tangent: the cache passes none")
-        if t.numel() and (t.stride(2) != 1 or self_overlapping(t)):
-            raise ValueError(f"{name} with strides {t.stride()} cannot be written: adjacent features, no element twice")
+        if t.numel() and (t.stride(2) != 1 or self_overlapping(t) or t.is_neg()):
+            raise ValueError(f"{name} with strides {t.stride()}{' and a lazy sign' if t.is_neg() else ''} cannot be written: adjacent features, no "
+                             "element twice")

@@ -117,8 +117,10 @@ def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, q, k,
 
 
 def _readable(t):
-    if t is not None and t._is_zerotensor():         # zeros that torch keeps without memory (tangents)
-        t = t.clone()
+    if t is not None:
+        if t._is_zerotensor():                       # zeros that torch keeps without memory (tangents)
+            t = t.clone()
+        t = t.resolve_neg()                          # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
     return t if t is None or (t.stride(-1) == 1 and (t.dim() <= 4 or _layout(t) is not None)) else t.contiguous()
 
 
@@ -229,8 +231,8 @@ class Rotary(nn.Module):
                 raise RuntimeError(f"{name} requires a gradient: apply_ is not differentiable, call the module instead")
             if has_tangent(t):
                 raise RuntimeError(f"{name} carries a tangent: apply_ is not differentiable, call the module instead")
-            if t.numel() and (t.stride(-1) != 1 or _layout(t) is None or self_overlapping(t)):
-                raise ValueError(f"{name} with strides {t.stride()} cannot be turned in place")
+            if t.numel() and (t.stride(-1) != 1 or _layout(t) is None or self_overlapping(t) or t.is_neg()):
+                raise ValueError(f"{name} with strides {t.stride()}{' and a lazy sign' if t.is_neg() else ''} cannot be turned in place")
         if k is not None and overlapping(q, k):
             raise ValueError("q and k are the same memory, or share some of it")
         overwritten(q, k)
