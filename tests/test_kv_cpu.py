@@ -8,6 +8,7 @@ import os
 import random
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
@@ -528,3 +529,20 @@ def test_lazily_negated_views(launches):
                  lambda: _call("read", out=(negated(2, 2, 32), torch.zeros(2, 2, 32)))):
         with pytest.raises(ValueError, match="lazy sign"):
             call()
+
+
+def test_overlapping_across_storages():
+    """Memory that two storages share (another library's buffer, taken over twice)."""
+    buf = np.zeros((3, 6, 32), np.float32)
+    a, b = torch.from_numpy(buf[:2]), torch.from_numpy(buf[1:])
+    assert a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr()
+    assert _lib.overlapping(a, b) and _lib.overlapping(b, a) and not _lib.overlapping(a[:1], b)
+    with pytest.raises(ValueError, match="share memory"):
+        _call("attend", q=a, out=b)
+    rng = random.Random(2)
+    flat = np.zeros(3000, np.float32)
+    for _ in range(300):
+        lo, hi = rng.randrange(2000), rng.randrange(2000)
+        n, m = rng.randint(1, 900), rng.randint(1, 900)
+        x, y = torch.from_numpy(flat[lo:lo + n]), torch.from_numpy(flat[hi:hi + m])
+        assert _lib.overlapping(x, y) == (lo < hi + m and hi < lo + n)

@@ -240,14 +240,15 @@ def self_overlapping(t):
 
 
 def overlapping(a, b):
-    """Whether some element of a shares memory with one of b (tensors of one element size): exact, also for pieces of one buffer's rows.
+    """Whether some element of a shares memory with one of b (tensors of one element size on one device): exact, also for pieces of one
+    buffer's rows, and whatever storages they belong to.
 
     Elements meet where sum(i * stride of a) - sum(j * stride of b) is the distance of the two; largest strides first, few
     multiples of each leave a rest that the smaller ones can make up."""
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or a.numel() == 0 or b.numel() == 0:
+    if a.numel() == 0 or b.numel() == 0:
         return False
     size = a.element_size()
-    ahead = b.data_ptr() - a.data_ptr()
+    ahead = b.data_ptr() - a.data_ptr()                 # (addresses: tensors of different storages may lie in the same memory)
     u, v = a.stride(), b.stride()
     if len(u) == len(v) > 2 and u[:-2] == v[:-2] and u[-3] > 0 and ahead % size == 0 and all(s % u[-3] == 0 for s in u[:-3]):
         # side by side in the rows of one buffer (queries and keys of one projection): told without what follows
