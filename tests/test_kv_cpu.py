@@ -546,3 +546,11 @@ def test_overlapping_across_storages():
         n, m = rng.randint(1, 900), rng.randint(1, 900)
         x, y = torch.from_numpy(flat[lo:lo + n]), torch.from_numpy(flat[hi:hi + m])
         assert _lib.overlapping(x, y) == (lo < hi + m and hi < lo + n)
+
+
+def test_a_table_of_one_block_each_has_any_strides(launches):
+    table = torch.arange(2, dtype=torch.int32)[None].t()
+    assert table.shape == (2, 1) and table.stride() == (1, 2)
+    _call("attend", table=table)
+    at = launches[0][1].index(table.data_ptr())
+    assert launches[0][1][at + 1] == 1                       # rows of the table one entry apart

@@ -83,7 +83,7 @@ class KVCache:
         """Checks the batch's description; returns the entry points' arguments (table, its stride, positions, offsets), then
         (sequences, width, rows of a sequence at most)."""
         shape = table.shape
-        if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or table.stride(1) != 1:
+        if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or (table.stride(1) != 1 and shape[1] > 1):
             raise ValueError(f"table: {table.dtype} {tuple(shape)}, not int32 [sequences, blocks] with adjacent blocks")
         n, width = shape
         at = self._numbers(what, positions, n)
