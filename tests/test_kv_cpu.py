@@ -554,3 +554,50 @@ def test_a_table_of_one_block_each_has_any_strides(launches):
     _call("attend", table=table)
     at = launches[0][1].index(table.data_ptr())
     assert launches[0][1][at + 1] == 1                       # rows of the table one entry apart
+
+
+UNITS = r'''
+#include <stdlib.h>
+#include "kv_layout.h"
+using namespace vamd;
+int main() {
+    // units are those that spans are found in
+    for (int unit = 64; unit <= 256; unit *= 2) for (int start = -2; start < 300; start += 7) for (int n = 0; n < 700; n += 9) {
+        int hit = 0;
+        for (int j = 0; j < 20; ++j) {
+            const KvSpan s = kv_span(start, n, ((start < 0 ? 0 : start) / unit + j) * (int64_t)unit, unit);
+            hit += s.hi > s.lo;
+        }
+        if (hit != kv_units(start, n, unit)) return 1;
+    }
+    if (kv_units(2147483647, 2147483647, 64) != 33554433) return 2;
+    // a batch's units fit into the launch, however its rows lie; without a bound the launch goes by the rows
+    srand(1);
+    for (int trial = 0; trial < 3000; ++trial) {
+        const int B = 1 + rand() % 70, unit = 64 << rand() % 3;
+        int64_t rows = 0, units = 0;
+        int most = 0;
+        for (int b = 0; b < B; ++b) {
+            const int n = rand() % 3 ? rand() % 4 : rand() % 3000;
+            rows += n;
+            most = n > most ? n : most;
+            units += kv_units(rand() % 1000, n, unit);
+        }
+        const KvUnits known = kv_io_units(true, B, rows, most, unit), open = kv_io_units(true, B, rows, (int)rows, unit);
+        if (units > known.count || units > open.count) return 3;
+        if (open.count > kKvListed * (rows / unit + 2 * B)) return 4;
+    }
+    const KvUnits u = kv_io_units(true, 256, 1 << 20, 1 << 20, 64), each = kv_io_units(false, 256, 1 << 20, 1 << 12, 64);
+    if (!u.listed || u.count != (1 << 14) + 512 || each.listed || each.count != 256 * 65) return 5;
+    return 0;
+}
+'''
+
+
+def test_units_of_a_batch(tmp_path):
+    src = tmp_path / "units.hip"
+    src.write_text(UNITS)
+    exe = str(tmp_path / "units")
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-I",
+                    os.path.join(ROOT, "vision_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True)
+    assert subprocess.run([exe]).returncode == 0

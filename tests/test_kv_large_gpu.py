@@ -57,3 +57,34 @@ def test_attention_of_more_than_2_to_32_threads():
     out = c.attend(q[torch.arange(B, device=DEV) % 7], table, lengths)
     want = c.attend(q, table[:7], lengths[:7])
     assert torch.equal(out, want[torch.arange(B, device=DEV) % 7])
+
+
+@pytest.mark.parametrize("block", [64, 256])
+def test_append_and_read_go_by_the_rows_there_are(block):
+    """Many ragged prompts of unknown length: by sequences times rows this call would not fit into any launch."""
+    B, H, D = 4096, 12, 16
+    counts = [(b * 37) % 1024 if b % 5 else 0 for b in range(B)]
+    starts = [-1 if b % 11 == 10 else (b * 13) % 100 for b in range(B)]
+    rows = sum(counts) + 9                                   # nine that belong to no sequence
+    offsets = [0]
+    for c in counts:
+        offsets.append(offsets[-1] + c)
+    assert B * (rows // block) * 2 * H > 2 ** 31 or block == 256
+    width = (1024 + 100 + block - 1) // block + 1
+    table = torch.randperm(B * width, device=DEV).to(torch.int32).view(B, width)
+    k, v = torch.randn(rows, H, D, device=DEV), torch.randn(rows, H, D, device=DEV)
+    off, start = i32(offsets), i32(starts)
+    caches = [KVCache(B * width, H, D, block=block, format="int8", device=DEV) for _ in range(2)]
+    caches[0].append(k, v, table, start, offsets=off)
+    caches[1].append(k, v, table, start, offsets=off, most=max(counts))
+    for name in ("codes_k", "codes_v", "scales_k", "scales_v"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
+    out = [tuple(torch.full((rows, H, D), 7.0, device=DEV) for _ in "kv") for _ in caches]
+    caches[0].read(table, start, rows, offsets=off, out=out[0])
+    caches[1].read(table, start, rows, offsets=off, most=max(counts), out=out[1])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    owned = torch.cat([torch.full((c,), s >= 0) for c, s in zip(counts, starts)] + [torch.zeros(9, dtype=torch.bool)]).to(DEV)
+    assert (out[0][0][~owned] == 7).all() and (out[0][0][owned] != 7).any(1).any(1).all()
+    few = caches[0].read(table, start, rows, offsets=off, most=3, out=tuple(torch.full((rows, H, D), 7.0, device=DEV) for _ in "kv"))
+    at = torch.cat([torch.arange(c) for c in counts] + [torch.full((9,), 9)]).to(DEV)
+    assert torch.equal(few[0], torch.where((at < 3)[:, None, None], out[0][0], 7.0))

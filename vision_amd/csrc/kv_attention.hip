@@ -75,10 +75,9 @@ __device__ __forceinline__ int kv_length(const KvAttendArgs& a, int b) {
     return n > room ? (int)room : n;
 }
 
-// Whose is tile number `tile` among those that the sequences really have, one sequence after the other?  Gives the sequence and the tile's
-// number in it, or false behind the last one.  64 sequences at a time, by the whole wave.
+// The sequence of tile number `tile` and the tile's number in it, or false behind the last one.
 //
-// Walked over by `most` instead, the tiles that short sequences do not have lie between the others in a regular pattern that leaves
+// Only tiles that there are have numbers.  Walked over by `most` instead, the tiles that short sequences do not have lie between the others in a regular pattern that leaves
 // whole CUs idle: prompts of 4096 and 925 tokens 435 us, of 4096 alone 264.
 __device__ __forceinline__ bool kv_whose_tile(const KvAttendArgs& a, int lane, int& tile, int& b) {
     if (!a.offsets || a.tiles == 1) {
@@ -86,25 +85,12 @@ __device__ __forceinline__ bool kv_whose_tile(const KvAttendArgs& a, int lane, i
         tile -= b * a.tiles;
         return b < a.sequences;
     }
-    for (int b0 = 0; b0 < a.sequences; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < a.sequences) n = (kv_rows(a.offsets, b0 + lane, a.rows, a.most).count * a.group + a.tile_rows - 1) / a.tile_rows;
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(upto, o, 64);
-            upto += lane >= o ? t : 0;
-        }
-        const uint64_t behind = __ballot(upto > tile);
-        if (behind) {
-            const int l = __ffsll((unsigned long long)behind) - 1;
-            b = __builtin_amdgcn_readfirstlane(b0 + l);
-            tile = __builtin_amdgcn_readfirstlane(tile - __shfl(upto - n, l, 64));
-            return true;
-        }
-        tile -= __shfl(upto, 63, 64);
-    }
-    return false;
+    uint32_t number = (uint32_t)tile;
+    const bool found = kv_whose(a.sequences, lane, [&](int s) {
+        return (kv_rows(a.offsets, s, a.rows, a.most).count * a.group + a.tile_rows - 1) / a.tile_rows;
+    }, number, b);
+    tile = (int)number;
+    return found;
 }
 
 __device__ __forceinline__ float kv_over_groups_max(float v) {           // over the four lanes that hold one query's keys

@@ -26,6 +26,7 @@ typedef __attribute__((ext_vector_type(2))) uint32_t kv_u32x2;
 typedef __attribute__((ext_vector_type(4))) uint32_t kv_u32x4;
 
 constexpr int kKvGroup = 64;                  // tokens of a group
+constexpr int kKvListed = 4;                  // see kv_io_units
 constexpr int kKvMinExp = -110, kKvMaxExp = 122;
 
 // byte of (token 0..63 of the group, feature d) for D features
@@ -102,6 +103,48 @@ __host__ __device__ __forceinline__ KvSpan kv_span(int64_t start, int count, int
     const int64_t lo = start > base ? start - base : 0, end = start + count - base;
     const int hi = end < 0 ? 0 : end < unit ? (int)end : unit;
     return KvSpan{lo < unit ? (int)lo : unit, hi};
+}
+// Units (blocks or groups) that rows at start .. start + count - 1 reach into.
+__host__ __device__ __forceinline__ int kv_units(int64_t start, int count, int unit) {
+    return start < 0 || count <= 0 ? 0 : (int)((start + count - 1) / unit - start / unit + 1);
+}
+// How the units of a packed batch are numbered.  By `touched`, which `most` rows reach at worst: unit number / touched of a sequence's, no
+// search, but numbers that short sequences lack.  Or (listed) one sequence's units after the other's, as kv_whose finds them: the
+// packed rows bound their number, whatever `most` says.  The search costs each workgroup a pass over the sequences before its own, empty
+// workgroups cost their launch; written and read back by `touched` / listed (8 heads of 128 features, us): 256 prompts up to 256,
+// known to be 67 + 34 / 92 + 45, unknown 1866 + 1340 / 92 + 45; 1000 up to 64, known 161 + 59 / 427 + 188, unknown 7073 + 5075 / 427 + 188; 255 tokens beside a
+// prompt of 4000 270 + 182 / 49 + 22 (28 numbers by `touched` for each listed one); 8 prompts up to 4096, known, 33 + 21 / 32 + 20.
+struct KvUnits {
+    int touched;
+    bool listed;
+    int64_t count;               // unit numbers a launch has to cover
+};
+__host__ __device__ __forceinline__ KvUnits kv_io_units(bool packed, int64_t sequences, int64_t rows, int most, int unit) {
+    const int touched = (int)(((int64_t)most + unit - 2) / unit + 1);
+    const int64_t each = sequences * touched, listed = rows / unit + 2 * sequences;
+    return packed && each > kKvListed * listed ? KvUnits{touched, true, listed} : KvUnits{touched, false, each};
+}
+// Whose is unit `number` among those that the sequences have, units_of(b) of them each, one sequence after the other?  Gives the
+// sequence and the unit's number in it, or false behind the last one.  64 sequences at a time, by the whole wave.
+template <typename F> __device__ __forceinline__ bool kv_whose(int sequences, int lane, F units_of, uint32_t& number, int& b) {
+    for (int b0 = 0; b0 < sequences; b0 += 64) {
+        const uint32_t n = b0 + lane < sequences ? (uint32_t)units_of(b0 + lane) : 0u;
+        uint32_t upto = n;                                   // (64 of up to 2^25 + 1: within 32 bits)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(upto, o, 64);
+            upto += lane >= o ? t : 0;
+        }
+        const uint64_t behind = __ballot(upto > number);
+        if (behind) {
+            const int l = __ffsll((unsigned long long)behind) - 1;
+            b = __builtin_amdgcn_readfirstlane(b0 + l);
+            number = (uint32_t)__builtin_amdgcn_readfirstlane((int)(number - __shfl(upto - n, l, 64)));
+            return true;
+        }
+        number -= __shfl(upto, 63, 64);
+    }
+    return false;
 }
 // The cache's block behind block `blk` of sequence b, or -1: behind the table's end, or a hole.
 __host__ __device__ __forceinline__ int kv_page(const int32_t* table, int64_t stride, int width, int blocks, int b, int64_t blk) {

@@ -26,7 +26,23 @@ struct KvIoArgs {
     const int32_t* offsets;
     int64_t rows;
     int sequences, heads, D, block, width, blocks, most, touched;
+    bool listed;                 // see KvUnits
 };
+
+// Unit number `id` of a launch: sequence b's j-th, or false where there is none.
+__device__ __forceinline__ bool kv_io_unit(const KvIoArgs& a, int64_t id, int unit, int& j, int& b) {
+    if (a.listed) {
+        uint32_t number = (uint32_t)id;
+        const bool found = kv_whose(a.sequences, (int)(threadIdx.x & 63), [&](int s) {
+            return kv_units(a.start[s], kv_rows(a.offsets, s, a.rows, a.most).count, unit);
+        }, number, b);
+        j = (int)number;
+        return found;
+    }
+    j = (int)(id % a.touched);
+    b = (int)(id / a.touched);
+    return b < a.sequences;
+}
 
 template <typename T, bool ALIGNED> __device__ __forceinline__ Vec16<T> kv_load16(const T* p) {
     if (ALIGNED) return *(const Vec16<T>*)p;
@@ -91,8 +107,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     id /= a.heads;
     const int kv = (int)(id & 1);
     id >>= 1;
-    const int j = (int)(id % a.touched), b = (int)(id / a.touched);
-    if (b >= a.sequences) return;
+    int j, b;
+    if (!kv_io_unit(a, id, a.block, j, b)) return;
     const int64_t start = a.start[b];
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int64_t blk = start / a.block + j, base = blk * a.block;
@@ -338,8 +354,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvIoArgs a) {
     id /= a.heads;
     const int kv = (int)(id & 1);
     id >>= 1;
-    const int j = (int)(id % a.touched), b = (int)(id / a.touched);
-    if (b >= a.sequences) return;
+    int j, b;
+    if (!kv_io_unit(a, id, kKvGroup, j, b)) return;
     const int64_t start = a.start[b];
     const KvRows rows = kv_rows(a.offsets, b, a.rows, a.most);
     const int64_t base = (start / kKvGroup + j) * kKvGroup;
@@ -417,9 +433,11 @@ static int kv_io_args(KvIoArgs& a, const char* name, const void* codes_k, const 
     a.width = width;
     a.blocks = blocks;
     a.most = most;
-    a.touched = (int)(((int64_t)most + unit - 2) / unit + 1);    // blocks or groups that `most` rows reach at worst
-    grid = (int64_t)sequences * a.touched * 2 * heads;
-    VAMD_REQUIRE((double)sequences * a.touched * 2 * heads <= kGridMost, "%s: %d sequences of up to %d rows and %d heads are too many for one call", name, sequences, most, heads);
+    const KvUnits units = kv_io_units(offsets != nullptr, sequences, rows, most, unit);
+    a.touched = units.touched;
+    a.listed = units.listed;
+    grid = units.count * 2 * heads;
+    VAMD_REQUIRE((double)units.count * 2 * heads <= kGridMost, "%s: %d sequences of up to %d rows and %d heads are too many for one call", name, sequences, most, heads);
     return 0;
 }
 static bool kv_aligned(const KvIoArgs& a, const void* p, const void* q, int dtype) {

@@ -14,8 +14,8 @@ for its values; a block's scale starts with the write of its first token and nev
 Rows k, v [rows, kv_heads, head_dim], q and out [rows, heads, head_dim] (heads a multiple of kv_heads; head h reads key head
 h // (heads // kv_heads)) are float32 or bfloat16 with any strides and adjacent features; packed one sequence after the other:
 sequence b owns rows offsets[b] .. offsets[b+1]-1 (`offsets` int32, [sequences + 1]), or without `offsets` rows / sequences each.
-`most` bounds the rows of a sequence where the caller knows it: launches are sized by it (default: all rows), rows of a sequence beyond
-it are left out.  `start`, `lengths`: int32, [sequences], on the GPU; nothing
+`most` bounds the rows of a sequence where the caller knows it (default: all rows); rows of a sequence beyond it are left out.  Launches
+are sized by it and by the rows there are: without it, finding whose rows a workgroup takes costs many short sequences some time.  `start`, `lengths`: int32, [sequences], on the GPU; nothing
 is copied to the host, so all of it can be captured into a graph.  Rows behind the last sequence are neither read nor written (in a
 result that the call allocates they hold nothing in particular).
 
