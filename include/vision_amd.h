@@ -541,7 +541,8 @@ int vamd_kv_read(const void* codes_k, const void* codes_v, const float* scales_k
 /* o = softmax(scale * q k^T) v over the first lengths[b] tokens of each sequence; q, o: [rows][heads * group][dim], query head h
  * reads key head h / group.  A sequence's queries are its last tokens: query i of n has position lengths[b] - n + i.  causal: it sees
  * keys up to its position, with window > 0 only the last `window` of them and the first `sinks`; else all.  Tokens in
- * holes are not seen; a query that sees nothing gives zeros.  `longest` (a bound of the lengths) only steers how the work is
+ * holes are not seen; a query that sees nothing gives zeros.  Results are finite for finite cached values of any size; a query's
+ * products with the codes (up to 448 and 127) are summed in fp32 before the scales, so |q| * 448 * dim has to stay below 2^128.  `longest` (a bound of the lengths) only steers how the work is
  * cut.  most * group: up to 2^28.  workspace: vamd_kv_attend_workspace bytes (may be 0), 16-byte aligned.
  * vamd_kv_attend_tile: rows (queries x heads of one key head) that a workgroup of such a call takes, 16, 64 or 128. */
 int vamd_kv_attend_tile(int64_t rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window,

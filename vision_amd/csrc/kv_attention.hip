@@ -35,7 +35,7 @@ struct KvAttendArgs {
     const int32_t* lengths;
     const int32_t* offsets;
     int64_t rows;
-    float* part;                 // [tiles of all sequences][heads][tile rows][splits][D] outputs, then [..][splits][2] maximum and sum
+    float* part;                 // [tiles of all sequences][heads][tile rows][splits][D] normalised outputs, then [..][splits][2] maximum and sum
     float* part_ml;
     float scale2;                // scale * log2(e)
     int sequences, most, heads, group, D, block_shift, width, blocks, window, sinks, causal, tiles, all_tiles, tile_rows, splits, q_aligned, o_aligned;
@@ -101,6 +101,16 @@ __device__ __forceinline__ float kv_over_groups_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
+// Values up to the largest float.  At a block whose values' scale is above 2^40 (a `big` one) a row's reference goes where the
+// probabilities until now (their `sum`, relative to m) come to less than 1/2, and those of this group's 64 keys (up to `top`) to 1/2 at
+// most: the output is then no larger than the largest value, whatever the number of keys.  For the same reason results are
+// normalised before they are joined, and joined by shares that sum to 1.
+constexpr int kKvBig = 40;
+__device__ __forceinline__ float kv_big_reference(float m, float sum, float top) {
+    return fmaxf(m + (float)((int)(__float_as_uint(sum) >> 23) - 125), top + 7.f);
+}
+__device__ __forceinline__ float kv_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }                    // (a row that sees nothing is zero)
+
 __device__ __forceinline__ float kv_finite(float m) { return m == -INFINITY ? 0.f : m; }
 
 // v as the sum of N bf16 numbers, the largest first
@@ -286,7 +296,9 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][i]);
         top = kv_over_groups_max(top);
-        const float m_new = fmaxf(m, top), m_use = kv_finite(m_new);
+        float m_new = fmaxf(m, top);
+        if ((int)(__float_as_uint(v_scale) >> 23) - 127 > kKvBig) m_new = kv_big_reference(m, kv_over_groups_sum(l), top);
+        const float m_use = kv_finite(m_new);
         if (__any(m_new != m)) {
             const float alpha = __builtin_amdgcn_exp2f(m - m_use);
             l *= alpha;
@@ -342,6 +354,13 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
         next = after;
     }
     l = kv_over_groups_sum(l);
+    {
+        const float inv = kv_inverse(l);
+#pragma unroll
+        for (int t = 0; t < C * 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][i] *= inv;
+    }
 
     // the four waves' results: 2 and 3 hand theirs to 0 and 1, then 1 to 0
     float* box_ml = lds + 2 * 64 * C * 16;
@@ -359,9 +378,10 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
             const float* box = lds + wave * 64 * C * 16;
             const float m2 = box_ml[(wave * 64 + lane) * 2], l2 = box_ml[(wave * 64 + lane) * 2 + 1];
             const float m_new = fmaxf(m, m2), m_use = kv_finite(m_new);
-            const float f1 = __builtin_amdgcn_exp2f(m - m_use), f2 = __builtin_amdgcn_exp2f(m2 - m_use);
+            const float w1 = l * __builtin_amdgcn_exp2f(m - m_use), w2 = l2 * __builtin_amdgcn_exp2f(m2 - m_use);
             m = m_new;
-            l = l * f1 + l2 * f2;
+            l = w1 + w2;
+            const float inv = kv_inverse(l), f1 = w1 * inv, f2 = w2 * inv;
 #pragma unroll
             for (int t = 0; t < C * 4; ++t) {
                 const kv_f32x4 o = *(const kv_f32x4*)(box + (t * 64 + lane) * 4);
@@ -384,14 +404,13 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
         }
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;                          // a row that sees nothing is zero
     T* o = (T*)a.o + (rows.first + tok) * a.o_tok + head * a.o_head;
 #pragma unroll
     for (int t = 0; t < C * 4; ++t) {
         if (t >= S) continue;
         T v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = from_f<T>(acc[t][i] * inv);
+        for (int i = 0; i < 4; ++i) v[i] = from_f<T>(acc[t][i]);
         if (a.o_aligned) {
             if (sizeof(T) == 4) *(kv_u32x4*)(o + t * 16 + g * 4) = *(const kv_u32x4*)v;
             else *(kv_u32x2*)(o + t * 16 + g * 4) = *(const kv_u32x2*)v;
@@ -630,7 +649,7 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
                           (a.window > 0 && k0 <= p_last - a.window && k0 + kKvGroup > a.sinks);
         // 2^e = v_scale is added to the exponents unless it is so far from 1 that probabilities could leave the range of a float
         const int v_exp = (int)(__float_as_uint(v_scale) >> 23) - 127;
-        const bool fold = v_exp >= -40 && v_exp <= 40;
+        const bool fold = v_exp >= -40 && v_exp <= kKvBig;
         const float v_add = fold ? (float)v_exp : 0.f, v_undo = fold ? __uint_as_float((uint32_t)(127 - v_exp) << 23) : 1.f;
         const int k1 = k0 + kh0 * 32 + hh * 4;               // token of the lane's first score
         if (edge) {
@@ -650,8 +669,9 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kh][i]);
         top = kv_over_halves_max(top) * f;
-        if (__any(top > m + 8.f)) {
-            const float m_new = top > m + 8.f ? top : m;
+        const bool big = v_exp > kKvBig;
+        if (__any(top > m + 8.f) || big) {
+            const float m_new = big ? kv_big_reference(m, kv_over_halves_sum(l), top) : top > m + 8.f ? top : m;
             const float alpha = __builtin_amdgcn_exp2f(m - kv_finite(m_new));
             l *= alpha;
 #pragma unroll
@@ -718,7 +738,7 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         }
         if (more) stage(buf ^ 1);
     }
-    float total = kv_over_halves_sum(l);
+    float total = kv_over_halves_sum(l), inv = kv_inverse(total);
     if constexpr (KW == 2) {
         // the waves of the keys' second halves hand theirs to those of the first: [wave_r][register][lane]
         __syncthreads();
@@ -727,20 +747,24 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) box[(t * 16 + i) * 64] = acc[t][i];
+                for (int i = 0; i < 16; ++i) box[(t * 16 + i) * 64] = acc[t][i] * inv;
             box[DT * 16 * 64] = m;
             box[(DT * 16 + 1) * 64] = total;
         }
         __syncthreads();
         if (kh0 == 1) return;
         const float m2 = box[DT * 16 * 64], m_new = fmaxf(m, m2);
-        const float f1 = __builtin_amdgcn_exp2f(m - kv_finite(m_new)), f2 = __builtin_amdgcn_exp2f(m2 - kv_finite(m_new));
+        const float w1 = __builtin_amdgcn_exp2f(m - kv_finite(m_new));
+        const float w2 = box[(DT * 16 + 1) * 64] * __builtin_amdgcn_exp2f(m2 - kv_finite(m_new));
         m = m_new;
-        total = total * f1 + box[(DT * 16 + 1) * 64] * f2;
+        total = total * w1 + w2;
+        inv = kv_inverse(total);
+        const float f1 = w1 * inv, f2 = w2 * inv;            // (this wave's output is not normalised yet, the other's is)
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[t][i] = acc[t][i] * f1 + box[(t * 16 + i) * 64] * f2;
+        inv = 1.f;
     }
     if (!live) return;
     if (a.splits > 1) {
@@ -751,14 +775,14 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (t * 2 + (i >> 1) < S)
-                    *(kv_f32x4*)(part + t * 32 + i * 8 + hh * 4) = kv_f32x4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+                    *(kv_f32x4*)(part + t * 32 + i * 8 + hh * 4) =
+                        kv_f32x4{acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv};
         if (hh == 0) {
             a.part_ml[at * 2] = m;
             a.part_ml[at * 2 + 1] = total;
         }
         return;
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
     T* o = (T*)a.o + (rows.first + tok) * a.o_tok + head * a.o_head;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -813,7 +837,7 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
         const int s = i * 64 + lane;
         const float m0 = s < used ? ml[2 * s] : -INFINITY, l0 = s < used ? ml[2 * s + 1] : 0.f;
         const float m1 = wave_max(m0), w = __builtin_amdgcn_exp2f(m0 - kv_finite(m1));
-        weight[s] = w;                                           // relative to the largest of its 64 shares
+        weight[s] = l0 * w;                                      // relative to the largest of its 64 shares
         const float l1 = wave_sum(l0 * w);
         if (lane == 0) {
             box_m[i] = m1;
@@ -828,6 +852,9 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
         f[i] = __builtin_amdgcn_exp2f(box_m[i] - m);
         l += box_l[i] * f[i];
     }
+    l = kv_inverse(l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] *= l;                       // shares sum to 1
     const int quads = a.D >> 2, lines = kKvJoin / quads;         // lanes of a row; rows (shares) read at once
     const int line = tid / quads, d = tid % quads * 4;
     kv_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -847,7 +874,7 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
     for (int e = tid; e < a.D; e += kKvJoin) {
         float v = 0.f;
         for (int i = 0; i < lines && i < used; ++i) v += box[(i * quads + (e >> 2)) * 4 + (e & 3)];
-        o[e] = from_f<T>(l == 0.f ? 0.f : v / l);
+        o[e] = from_f<T>(v);
     }
 }
 
