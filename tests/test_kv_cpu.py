@@ -601,3 +601,33 @@ def test_units_of_a_batch(tmp_path):
     subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-I",
                     os.path.join(ROOT, "vision_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True)
     assert subprocess.run([exe]).returncode == 0
+
+
+PIECES = r'''
+#include "kv_layout.h"
+using namespace vamd;
+int main() {
+    for (int D = 16; D <= 256; D += 16) for (int q = 0; q < 4 * D; ++q) {
+        int t, d, g;
+        kv_key_piece(q, D / 16, t, d);
+        for (int f = 0; f < 16; ++f) if (kv_key_at(t, d + f, D) != q * 16 + f) return 1;
+        kv_value_piece(q, g, d);
+        for (int i = 0; i < 16; ++i) if (kv_value_at(i / 4 * 16 + 4 * g + i % 4, d) != q * 16 + i) return 2;
+    }
+    // what a lane of the decoding kernel adds to a tile's first piece
+    for (int D = 64; D <= 256; D += 64) for (int lane = 0; lane < 64; ++lane) for (int c = 0; c < D / 64; ++c) for (int t = 0; t < 4; ++t)
+        if (kv_key_at(t * 16, c * 64, D) + lane * 16 != kv_key_at(t * 16 + (lane & 15), c * 64 + (lane >> 4) * 16, D)) return 3;
+    for (int lane = 0; lane < 64; ++lane) for (int s = 0; s < 16; ++s)
+        if (kv_value_at(0, s * 16) + lane * 16 != kv_value_at(4 * (lane >> 4), s * 16 + (lane & 15))) return 4;
+    return 0;
+}
+'''
+
+
+def test_the_layout_both_ways(tmp_path):
+    src = tmp_path / "pieces.hip"
+    src.write_text(PIECES)
+    exe = str(tmp_path / "pieces")
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-I",
+                    os.path.join(ROOT, "vision_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True)
+    assert subprocess.run([exe]).returncode == 0

@@ -224,14 +224,14 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int c = 0; c < C; ++c) kc[t * C + c] = load(p + (t * S + c * 4) * 256 + (c < C - 1 ? k_lane : k_lane_last));
+            for (int c = 0; c < C; ++c) kc[t * C + c] = load(p + kv_key_at(t * 16, c * 64, a.D) + (c < C - 1 ? k_lane : k_lane_last));
     };
     auto load_v = [&](int page, int x) {
         const uint8_t* p = bytes_of(1, page, x);
         vs = a.scales[1][at_of(page)];
 #pragma unroll
         for (int s = 0; s < 4 * C; ++s)
-            if (s < S) vc[s] = load(p + s * 1024 + k_lane);
+            if (s < S) vc[s] = load(p + kv_value_at(0, s * 16) + k_lane);
     };
     int x = begin + wave;
     int page = page_of(x), next = page_of(x + 4);
@@ -526,12 +526,13 @@ __global__ void __launch_bounds__(kKvTileThreads, DT <= (sizeof(T) == 4 ? 2 : 4)
         for (int i = 0; i < PIECES; ++i) {
             const int q = tid + i * kKvTileThreads;
             if (q < 64 * S) {
-                const int token = (q >> 4) / S * 16 + (q & 15), slab = (q >> 4) % S;
+                int token, kd, g, d;
+                kv_key_piece(q, S, token, kd);
+                kv_value_piece(q, g, d);
                 const kv_u32x4 kw = kv_as_loaded(st[0][i]);
-                *(kv_bf16x8*)(kb + ((slab * 2) * 64 + token) * 16) = kv_operand8<FMT>(kw[0], kw[1]);
-                *(kv_bf16x8*)(kb + ((slab * 2 + 1) * 64 + token) * 16) = kv_operand8<FMT>(kw[2], kw[3]);
+                *(kv_bf16x8*)(kb + ((kd >> 3) * 64 + token) * 16) = kv_operand8<FMT>(kw[0], kw[1]);
+                *(kv_bf16x8*)(kb + ((kd >> 3) * 64 + 64 + token) * 16) = kv_operand8<FMT>(kw[2], kw[3]);
                 if (FMT == VAMD_KV_INT8) __builtin_amdgcn_sched_barrier(0);  // one conversion's floats at a time
-                const int g = (q >> 4) & 3, d = (q >> 6) * 16 + (q & 15);
                 const kv_u32x4 vw = kv_as_loaded(st[1][i]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {

@@ -37,6 +37,17 @@ __host__ __device__ __forceinline__ int kv_value_at(int token, int d) {
     return (((d >> 4) * 4 + ((token >> 2) & 3)) * 16 + (d & 15)) * 16 + (token >> 4) * 4 + (token & 3);
 }
 
+// The other way round: what 16-byte piece q of a group holds.  Keys (S = D / 16 slabs): 16 features from d on of token t; values: of feature d,
+// tokens 16 tile + 4 g + 0 .. 3 of the four tiles.
+__host__ __device__ __forceinline__ void kv_key_piece(int q, int S, int& t, int& d) {
+    t = (q >> 4) / S * 16 + (q & 15);
+    d = (q >> 4) % S * 16;
+}
+__host__ __device__ __forceinline__ void kv_value_piece(int q, int& g, int& d) {
+    g = (q >> 4) & 3;
+    d = (q >> 6) * 16 + (q & 15);
+}
+
 // Four codes (a dword) as floats, and back.  Codes of finite blocks never exceed the largest code: no saturation is needed.
 template <int FMT> __device__ __forceinline__ kv_f32x4 kv_decode4(uint32_t w) {
     if (FMT == VAMD_KV_E4M3) {

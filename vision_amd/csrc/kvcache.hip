@@ -127,11 +127,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     const int f0 = lo / kKvGroup, f1 = (hi + kKvGroup - 1) / kKvGroup;          // groups with fresh tokens
     const int items = (f1 - f0) * (kv == 0 ? pieces : quads), per = kv == 0 ? 2 * HOLD : HOLD;
     const bool held = items <= per * nt;
-    auto key_place = [&](int i, int& g, int& q, int& t, int& d) {
+    auto key_place = [&](int i, int& g, int& t, int& d) {
         g = i / pieces;
-        q = i - g * pieces;
-        t = g * kKvGroup + (q >> 4) / S * 16 + (q & 15);
-        d = (q >> 4) % S * 16;
+        kv_key_piece(i - g * pieces, S, t, d);
+        t += g * kKvGroup;
     };
     auto value_place = [&](int i, int& g, int& t, int& p, int& gg, int& tt) {
         g = i / quads;
@@ -154,9 +153,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     if (held && kv == 0) {
 #pragma unroll
         for (int n = 0; n < 2 * HOLD; ++n) {
-            int g, q, t = hi, d = 0;
+            int g, t = hi, d = 0;
             const int i = tid + n * nt;
-            if (i < items) key_place(i + f0 * pieces, g, q, t, d);
+            if (i < items) key_place(i + f0 * pieces, g, t, d);
 #pragma unroll
             for (int e = 0; e < 2 * V8; ++e) {
                 Vec16<T> w = {};
@@ -228,8 +227,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     auto encode_quad = [&](const float (&v)[4][8], int e) {
         return dead ? 0u : kv_encode4<FMT>(fit(v[0][e]), fit(v[1][e]), fit(v[2][e]), fit(v[3][e]));
     };
+    auto key_at = [&](int g, int t, int d) { return codes + (int64_t)g * kKvGroup * D + kv_key_at(t & (kKvGroup - 1), d, D); };
     auto quad_at = [&](int g, int p, int gg, int tt) {
-        return codes + (int64_t)g * kKvGroup * D + (((p >> 1) * 4 + gg) * 16 + (p & 1) * 8) * 16 + tt * 4;
+        return codes + (int64_t)g * kKvGroup * D + kv_value_at(tt * 16 + gg * 4, p * 8);
     };
     // stores the fresh tokens of a quad (t ..): in a group that is fresh throughout the four lanes of the same features (tiles 0 .. 3) trade
     // dwords, so that each stores the 16 bytes of two features (with 4-byte stores 16 bytes apart 16000 tokens took 28 us, so 26);
@@ -265,10 +265,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
         const int groups = a.block / kKvGroup;
         if (kv == 0) {
             for (int i = tid; i < groups * pieces; i += nt) {
-                int g, q, t, d;
-                key_place(i, g, q, t, d);
+                int g, t, d;
+                key_place(i, g, t, d);
                 if (t >= lo && t < hi) continue;
-                kv_u32x4* to = (kv_u32x4*)(codes + (int64_t)g * kKvGroup * D) + q;
+                kv_u32x4* to = (kv_u32x4*)key_at(g, t, d);
                 kv_u32x4 w = *to;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = old ? kv_rescale4<FMT>(w[e], ratio) : 0u;
@@ -288,9 +288,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
     }
     if (kv == 0) {
         auto put = [&](int i, const float (&v)[16]) {
-            int g, q, t, d;
-            key_place(i + f0 * pieces, g, q, t, d);
-            if (t >= lo && t < hi) *((kv_u32x4*)(codes + (int64_t)g * kKvGroup * D) + q) = encode_key(v);
+            int g, t, d;
+            key_place(i + f0 * pieces, g, t, d);
+            if (t >= lo && t < hi) *(kv_u32x4*)key_at(g, t, d) = encode_key(v);
         };
         if (held) {
 #pragma unroll
@@ -302,8 +302,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
             }
         } else {
             for (int i = tid; i < items; i += nt) {
-                int g, q, t, d;
-                key_place(i + f0 * pieces, g, q, t, d);
+                int g, t, d;
+                key_place(i + f0 * pieces, g, t, d);
                 if (t < lo || t >= hi) continue;
                 float v[16], u[2][8];
                 kv_load8<T, ALIGNED>(x + t * tok + d, u[0]);
@@ -372,9 +372,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvIoArgs a) {
     if (kv == 0) {
         const int S = D >> 4, pieces = kKvGroup * S;
         for (int q = tid; q < pieces; q += nt) {
-            const int t = (q >> 4) / S * 16 + (q & 15), d = (q >> 4) % S * 16;
+            int t, d;
+            kv_key_piece(q, S, t, d);
             if (t < lo || t >= hi) continue;
-            const kv_u32x4 w = hole ? kv_u32x4{0, 0, 0, 0} : *((const kv_u32x4*)codes + q);
+            const kv_u32x4 w = hole ? kv_u32x4{0, 0, 0, 0} : *(const kv_u32x4*)(codes + kv_key_at(t, d, D));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const kv_f32x4 l = kv_decode4<FMT>(w[2 * e]), r = kv_decode4<FMT>(w[2 * e + 1]);
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvIoArgs a) {
         for (int q = tid; q < 16 * P; q += nt) {
             const int tt = q & 3, p = (q >> 2) % P, gg = (q >> 2) / P, t = tt * 16 + gg * 4;
             if (t + 4 <= lo || t >= hi) continue;
-            const uint8_t* from = codes + (((p >> 1) * 4 + gg) * 16 + (p & 1) * 8) * 16 + tt * 4;
+            const uint8_t* from = codes + kv_value_at(t, p * 8);
             float v[4][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
