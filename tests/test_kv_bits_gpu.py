@@ -1,9 +1,12 @@
-"""How many bits attention over the 8-bit cache keeps where there are few queries: all but the result's own rounding."""
+"""Attention over the 8-bit cache: how many bits a result keeps where there are few queries (all but its own rounding), and queries that are
+one row in memory for many tokens."""
 import pytest
 import torch
 
 import kv_plain
 from test_kv_attention_gpu import filled, i32, offsets_of, rnd
+from vision_amd import _lib
+from vision_amd._lib import lib
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +28,23 @@ def test_bf16_probabilities_keep_sixteen_bits(shape):
         bound = 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * (2.0 ** -16 + rel) * size + 1e-30
         worst = ((out[qo[b]:qo[b + 1]] - want).abs() / bound).max()
         assert worst <= 1, (b, L, float(worst))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("H,count", [(2, 1), (2, 50), (16, 70), (16, 200)])
+def test_expanded_queries(H, count, dtype):
+    """One row of queries for every token (a token stride of 0): every row is that of the same queries laid out; small and large tiles."""
+    D = 48
+    lengths = [250, 201]
+    c, table, k, v, off = filled(lengths, H, D, 64, "e4m3", 360)
+    t = _lib.F32 if dtype == torch.float32 else _lib.BF16
+    sequences = [0, 1] * (1 if H == 2 else 8)
+    tile = lib.vamd_kv_attend_tile(count * len(sequences), len(sequences), count, 250, H, 3, D, 0, 0, t)
+    assert tile == (16 if H == 2 else 128)
+    one = rnd((1, 3 * H, D), dtype, 369).expand(count * len(sequences), 3 * H, D)
+    lengths, table = i32([lengths[b] for b in sequences]), table[sequences].contiguous()
+    for kw in ({}, dict(window=30, sinks=2), dict(causal=False)):
+        out = c.attend(one, table, lengths, longest=250, **kw)
+        assert torch.equal(out, c.attend(one.contiguous(), table, lengths, longest=250, **kw))
+    # without the causal bound all tokens of a sequence see the same
+    assert torch.equal(out.view(len(sequences), count, 3 * H, D), out.view(len(sequences), count, 3 * H, D)[:, :1].expand(-1, count, -1, -1))
