@@ -631,3 +631,11 @@ def test_the_layout_both_ways(tmp_path):
     subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-host-only", "-O1", "-std=c++17", "-I",
                     os.path.join(ROOT, "vision_amd", "csrc"), str(src), "-o", exe], check=True, capture_output=True)
     assert subprocess.run([exe]).returncode == 0
+
+
+def test_rotary_refuses_keys_of_too_few_dimensions():
+    r, pos = Rotary(32), torch.tensor(3)
+    for k in (torch.zeros(32), torch.zeros(())):             # beside queries [heads, head_dim]
+        for call in (r, r.apply_):
+            with pytest.raises(ValueError, match="differ"):
+                call(pos, torch.zeros(4, 32), k)

@@ -191,7 +191,8 @@ class Rotary(nn.Module):
         if len(shape) < 2 or shape[-1] != self.head_dim:
             raise ValueError(f"q has shape {tuple(shape)}, not [..., heads, {self.head_dim}]")
         lead, index = shape[:-2], q.get_device()
-        if k is not None and (k.dtype != dtype or k.shape[-1] != self.head_dim or k.shape[:-2] != lead or k.get_device() != index):
+        if k is not None and (k.dtype != dtype or k.dim() != len(shape) or k.shape[-1] != self.head_dim or k.shape[:-2] != lead or
+                              k.get_device() != index):
             raise ValueError(f"q and k differ: {dtype} {tuple(shape)} on {q.device}, {k.dtype} {tuple(k.shape)} on {k.device}")
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"positions are {positions.dtype}: int32 or int64")
