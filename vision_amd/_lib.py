@@ -199,13 +199,14 @@ def call(name, *args):
 
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+_tracing, _modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
 _entries = {name: getattr(lib, name) for name in SIGNATURES}
 
 
 def call_on(device, name, *args):
     """The same on the current stream of `device` (its last argument), whichever device is current.  A kernel launched from here is
     invisible to what records torch's operators, whose program would return memory that nobody writes: refused there."""
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _tracing() is not None or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None):
         raise RuntimeError(f"{name} cannot be recorded by torch.jit.trace or make_fx: call it outside of the traced function")
     index = device.index
     if index == torch.cuda.current_device():
@@ -226,7 +227,7 @@ def overwritten(*tensors):
 
 def has_tangent(t):
     """Whether t is a dual number of forward-mode differentiation (whether or not it requires a gradient)."""
-    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def self_overlapping(t):
@@ -247,6 +248,10 @@ def overlapping(a, b):
     multiples of each leave a rest that the smaller ones can make up."""
     if a.numel() == 0 or b.numel() == 0:
         return False
+    u, v = a.untyped_storage(), b.untyped_storage()
+    at, to = u.data_ptr(), v.data_ptr()
+    if at != to and (at + u.nbytes() <= to or to + v.nbytes() <= at):
+        return False                                    # no memory in common, whatever of it they use
     size = a.element_size()
     ahead = b.data_ptr() - a.data_ptr()                 # (addresses: tensors of different storages may lie in the same memory)
     u, v = a.stride(), b.stride()

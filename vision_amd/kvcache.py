@@ -68,7 +68,8 @@ class KVCache:
             raise RuntimeError(f"{name} carries a tangent: the cache passes none")
         if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        t = t.resolve_neg()                              # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
+        if t.is_neg():
+            t = t.resolve_neg()                          # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
         return t if t.stride(2) == 1 else t.contiguous()
 
     def _numbers(self, name, t, size):

@@ -118,9 +118,8 @@ def _turn(positions, frequencies, amplitude, turned, interleaved, inverse, q, k,
 
 def _readable(t):
     if t is not None:
-        if t._is_zerotensor():                       # zeros that torch keeps without memory (tangents)
-            t = t.clone()
-        t = t.resolve_neg()                          # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
+        if t.is_neg():
+            t = t.resolve_neg()                      # a view whose sign torch keeps apart from the memory (tensor.conj().imag)
     return t if t is None or (t.stride(-1) == 1 and (t.dim() <= 4 or _layout(t) is not None)) else t.contiguous()
 
 
@@ -165,6 +164,7 @@ class _RotaryFn(torch.autograd.Function):
     def jvp(ctx, _positions, _frequencies, _how, tq, tk):
         # linear: a tangent is turned as its tensor is (forward: q and k both have one, or there is no other)
         turn = _RotaryFn.apply if torch.is_grad_enabled() else _turned
+        tq, tk = (t.clone() if t is not None and t._is_zerotensor() else t for t in (tq, tk))    # (zeros that torch keeps without memory)
         return turn(*ctx.saved_tensors, ctx.how, tq, tk)
 
 
