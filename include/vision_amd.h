@@ -533,7 +533,7 @@ int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, const void* v
                    const int32_t* start, const int32_t* offsets, int64_t rows, int sequences, int most, int heads, int dim,
                    int block, int width, int blocks, int format, int dtype, void* stream);
 /* Reads the values at positions start[b], start[b]+1, ... back into rows k, v [rows][heads][dim] (exact in fp32 and in bf16);
- * zeros for holes.  A sequence with start < 0 is left out. */
+ * zeros for holes and behind `width` blocks.  A sequence with start < 0 is left out: its rows keep what they held. */
 int vamd_kv_read(const void* codes_k, const void* codes_v, const float* scales_k, const float* scales_v, const int32_t* table,
                  int64_t table_stride, const int32_t* start, const int32_t* offsets, int64_t rows, int sequences, int most,
                  int heads, int dim, int block, int width, int blocks, int format, void* k, int64_t k_token, int64_t k_head,
@@ -543,7 +543,7 @@ int vamd_kv_read(const void* codes_k, const void* codes_v, const float* scales_k
  * keys up to its position, with window > 0 only the last `window` of them and the first `sinks`; else all.  Tokens in
  * holes are not seen; a query that sees nothing gives zeros.  Results are finite for finite cached values of any size; a query's
  * products with the codes (up to 448 and 127) are summed in fp32 before the scales, so |q| * 448 * dim has to stay below 2^128.  `longest` (a bound of the lengths) only steers how the work is
- * cut.  most * group: up to 2^28.  workspace: vamd_kv_attend_workspace bytes (may be 0), 16-byte aligned.
+ * cut.  A length beyond width * block is cut to that, one below 0 to 0, before positions are taken from it.  most * group: up to 2^28.  workspace: vamd_kv_attend_workspace bytes (may be 0), 16-byte aligned.
  * vamd_kv_attend_tile: rows (queries x heads of one key head) that a workgroup of such a call takes, 16, 64 or 128. */
 int vamd_kv_attend_tile(int64_t rows, int sequences, int most, int64_t longest, int heads, int group, int dim, int window,
                         int sinks, int dtype);

@@ -8,7 +8,7 @@
 //
 // kv_attend_rows_kernel: few queries (a decoding step).  A tile is up to 16 rows (query tokens x heads of one key head), so that
 // every code of the cache is read once for all heads that share it; bound by reading the cache (64 sequences of up to 4096, 8 key heads
-// of 128 features: 56 us, 4.7 TB/s).  Each of a workgroup's four
+// of 128 features: 56 us, 4.7 TB/s; of 256 features 112, 4.7; float32 queries 63, 4.2).  Each of a workgroup's four
 // waves takes every fourth group of 64 tokens of its share of the keys; codes go straight from global memory into MFMA
 // operand order (16 bytes a lane, 1 KB a wave and load) and become bf16 in registers: code values are exact there.  With the keys as the
 // rows of the first product a lane holds 16 scores of ONE query, and exactly the slots that the second product wants as its
@@ -135,9 +135,10 @@ __device__ __forceinline__ kv_u32x4 kv_as_loaded(kv_u32x4 w) {
     return w;
 }
 
-// C: 64-feature chunks of a head (the last one may be partly empty).  ONCE: one tile of rows, so that every code is read once, past the
-// caches' replacement (256 sequences up to 2000: 117 -> 103 us, 64 up to 4096 64 -> 56); with more tiles the others find them there
-// (two tiles: 67 us, 71 past it).
+// C: 64-feature chunks of a head (the last one may be partly empty).  ONCE: one tile of rows, so that a sequence's codes are read once, past
+// the caches' replacement (256 sequences up to 2000: 117 -> 103 us, 64 of 4160 107 -> 94); with more tiles the others find them there
+// (two tiles: 67 us, 71 past it).  Sequences that share the blocks of a common beginning lose nothing by it: 64 of 4160 tokens sharing 4096 49.8 us,
+// 49.2 without; 16 of 32832 sharing 32768 90.8, 89.8 without.
 template <typename T, int FMT, int C, bool ONCE>
 __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(const KvAttendArgs a) {
     constexpr int N = sizeof(T) == 4 ? 3 : 1, PN = sizeof(T) == 4 ? 3 : 2;       // bf16 pieces of a query, of a probability
@@ -440,8 +441,9 @@ __global__ void __launch_bounds__(256, C <= 2 ? 2 : 1) kv_attend_rows_kernel(con
 // scale goes into the exponent.
 //
 // Bound by the matrix cores, the exponentials and the LDS reads about alike (an operand is read once for 32 queries, 128 bytes a
-// clock): 30000 keys before 2048 queries of 32 heads, 128 features, 938 TFLOP/s; prompts of 4096 and 925 tokens behind
-// 1000 760 to 840, where causal tiles of unlike length leave some of the chip idle; a plain bf16 product of 8192^3 reaches 1234.
+// clock): 30000 keys before 2048 queries of 32 heads, 128 features, 940 TFLOP/s; prompts of 4096 and 925 tokens behind
+// 1000 714 (kernel trace, 301 us) to 818 (passes in a row, 263 us), where causal tiles of unlike length leave some of the chip idle; a
+// plain bf16 product of 8192^3 reaches 1234.
 //
 // DT: tiles of 32 features (the last may be half empty).
 __device__ __forceinline__ float kv_over_halves_max(float v) {               // over the two lanes that hold one query's keys
@@ -891,13 +893,13 @@ __global__ void __launch_bounds__(kKvJoin) kv_join_kernel(const KvAttendArgs a) 
 // than 128 features 256) workgroups of them: 128 rows from 512 workgroups on, 64 above 256, and only where a sequence has
 // more than 16 rows on average (255 sequences of 2 queries behind 1000, `most` given as 510: 109 us in tiles of 16, 164 of 64).
 // us with 8 key heads of 128 features and groups of 4 (16 / 64 / 128 rows): 2048 queries (512 tiles of 128) 150 / 92 / 75; up to 4 x 1024 behind 8000 keys 355 / 255 / 240; 4096
-// queries of 8 ungrouped heads of 64 features 84 / 71 / 86; 512 queries (128 tiles) 30 / 24 / 28; 16 x 30 behind 1000 (128) 26 / 34 / 41; 100
+// queries of 8 ungrouped heads of 64 features 84 / 71 / 86; 512 queries (128 tiles) 30 / 24 / 28; 16 of up to 30 behind up to 1000 (128) 26 / 34 / 41; 100
 // queries (32) 14 / 17 / 18.  float32 (three products): up to 2 x 2000 queries 202 / 218 / 163, up to 4 x 200 30 / 39 / 51.
 //
-// Then shares of the keys, until 512 workgroups have work.  Tiles of 16: no share less than 8 groups of 64 tokens.  One token of
-// 64 sequences of up to 4096 (8 key heads, 128 features): 56 us with 256 or 512, 60 with 768 or 1024 workgroups; of
-// one sequence of 131071: 37, 38, 41 and 42 us; 8 queries of 16 sequences of up to 8000 (two tiles): 80, 67, 57 and 62; 30
-// queries of 16 sequences behind 1000: 26, 26, 47 and 47.  Large tiles, whose partial results are many: only from 4 shares of 16 groups on
+// Then shares of the keys, until 512 workgroups have work.  Tiles of 16: no share less than 8 groups of 64 tokens.  us with 256 / 512 / 768 /
+// 1024 workgroups, three states in turn: one token of 64 sequences of up to 4096 (8 key heads, 128 features) 57 / 57 / 62 / 62; of one sequence
+// of 131071 37 / 39 / 42 / 42; of 16 windows of 2000 24 / 26 / 26 / 26; 4 queries of 16 sequences of up to 8000 48 / 45 / 51 / 49; 8 queries (two tiles) 87
+// / 71 / 74 / 69.  Large tiles, whose partial results are many: only from 4 shares of 16 groups on
 // (2048 queries as two shares 140 us, as one 71; 64 queries behind 60000 keys as 32 shares 104).
 struct KvPlan {
     int tile_rows, tiles, splits;    // tiles of a sequence of `most` rows
@@ -978,8 +980,8 @@ template <typename T, int FMT, int KW> static int kv_launch_tile(const KvAttendA
     return fail(VAMD_EUNSUPPORTED, "vamd_kv_attend: no kernel for %d features in float32", a.D);
 }
 
-// One wave per row, four or sixteen: so many that a lane reads about four shares.  32 rows of 256 shares: 12 us with four waves, 5.8 with
-// sixteen; 512 rows of 4 shares (128 features): 18 us with sixteen waves, 4 with one.
+// One wave per row, four or sixteen: so many that a lane reads about four shares.  32 rows of 256 shares: 12 us with four waves, 5.5 with
+// sixteen; 512 rows of 4 shares (128 features): 18 us with sixteen waves, 5.5 with one.
 template <typename T> static int kv_launch_join(const KvAttendArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.all_tiles * a.heads * kv_tile_fill(a.tiles, a.tile_rows, a.most, a.group));
     const int lanes = a.splits * (a.D / 4) / 4;

@@ -8,7 +8,8 @@
 //      32 bits and one rounding to the code: e4m3 codes only lose bits that fall below the smallest code, int8 codes round again;
 //   3. the rows as codes, from registers where a workgroup can hold them, else read again (from L2): x * 2^-e is exact, the code's
 //      rounding (to nearest, ties to even) is the only one.
-// Bound by memory: 16000 tokens of 8 heads and 128 features (int8, blocks of 128) 26 us written, 21 read back, 3.9 and 4.8 TB/s.  A block belongs to one sequence while it is written: no two
+// Bound by memory: 16000 tokens of 8 heads and 128 features (int8, blocks of 128) 29 us written, 21 read back, 3.4 and 4.6
+// TB/s.  A block belongs to one sequence while it is written: no two
 // workgroups of a call write the same bytes, nothing is added atomically, the result does not depend on any order.
 #include "kv_layout.h"
 
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvIoArgs a) {
         return codes + (int64_t)g * kKvGroup * D + kv_value_at(tt * 16 + gg * 4, p * 8);
     };
     // stores the fresh tokens of a quad (t ..): in a group that is fresh throughout the four lanes of the same features (tiles 0 .. 3) trade
-    // dwords, so that each stores the 16 bytes of two features (with 4-byte stores 16 bytes apart 16000 tokens took 28 us, so 26);
+    // dwords, so that each stores the 16 bytes of two features (with 4-byte stores 16 bytes apart 16000 tokens take 28 us where these take 26);
     // else whole dwords, or their bytes beside others that stay
     auto put_quad = [&](uint8_t* to, const float (&v)[4][8], int t) {
         const int group = t & ~(kKvGroup - 1), tt = (t >> 4) & 3;
@@ -488,8 +489,8 @@ extern "C" int vamd_kv_append(const void* k, int64_t k_token, int64_t k_head, co
     // One wave where a block gets at most 4 tokens (a decoding step: no barrier, more blocks a CU), else four.
     const int threads = most <= 4 ? 64 : 256;
     // What four waves hold in registers: blocks up to 16384 elements (64 or 128 tokens of 128 features) with HOLD 2, up to 32768 with 4
-    // (beyond that the rows are read twice).  16000 tokens of 8 heads, 128 features, written and read back: blocks of 128 tokens 53 us with
-    // 2, 66 with 4, 67 read twice; of 256 tokens 60 with 4, 71 read twice.
+    // (beyond that the rows are read twice).  16000 tokens of 8 heads, 128 features, written and read back in one pass: blocks of 128 tokens
+    // 53 us with 2, 66 with 4, 67 read twice; of 256 tokens 60 with 4, 71 read twice.
     if (block * dim <= 16384 || threads == 64) VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 2>););
     else VAMD_DISPATCH(dtype, "vamd_kv_append", KV_IO_LAUNCH(kv_append_kernel<T COMMA F COMMA A COMMA 4>););
     VAMD_LAUNCH_OK("kv_append");

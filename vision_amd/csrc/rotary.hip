@@ -12,7 +12,8 @@
 // Memory bound: every element is read and written once, in pieces of 16 bytes where the layout allows it.  One lane owns
 // 2 V features (V pairs' halves, or V whole pairs) of one token and walks over `per` heads of both tensors, so that the
 // angles of a token are computed once for `per` heads; neighbouring lanes own neighbouring pieces of a row.  16383 tokens of 32 + 8
-// heads of 128 features in bf16: 62 us, 5.4 TB/s (a large copy: 5.2); 4099 tokens of 16 + 16 heads of 96 in float32: 21 us, 4.8.
+// heads of 128 features in bf16: 65 us, 5.1 TB/s (a large copy: 5.2); 4099 tokens of 16 + 16 heads of 96 in float32: 29 us, 3.5 (21 us where
+// the inputs are still in the caches).
 #include "common.h"
 
 namespace vamd {

@@ -19,7 +19,8 @@ are sized by it and by the rows there are: without it, finding whose rows a work
 is copied to the host, so all of it can be captured into a graph.  Rows behind the last sequence are neither read nor written (in a
 result that the call allocates they hold nothing in particular).
 
-The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no gradient.
+The layout is the kernels' own (csrc/kv_layout.h); there is no CPU path and no gradient, backward or forward: tensors that require one or
+carry a tangent are refused.  A call cannot be recorded by torch.jit.trace or make_fx; `out` counts as modified in place.
 """
 import torch
 
@@ -124,7 +125,8 @@ class KVCache:
 
     def read(self, table, start, rows, offsets=None, most=None, dtype=torch.bfloat16, out=None):
         """(k, v): the values at positions start[b], start[b]+1, ... of each sequence, `rows` rows in all, exact in either dtype; zeros
-        in holes.  `out`: two tensors [rows, kv_heads, head_dim] to write into; rows of no sequence keep what they held."""
+        in holes and behind the table's end.  `out`: two tensors [rows, kv_heads, head_dim] to write into; rows of no sequence, beyond `most`
+        or of a sequence with start < 0 keep what they held (in a result that the call allocates they hold nothing in particular)."""
         if out is None:
             if dtype not in _TYPES:
                 raise TypeError(f"dtype {dtype}: float32 or bfloat16")
@@ -151,7 +153,7 @@ class KVCache:
     def attend(self, q, table, lengths, offsets=None, most=None, longest=None, scale=None, causal=True, window=0, sinks=0, out=None):
         """softmax(scale * q k^T) v over the first lengths[b] tokens of each sequence, whose queries are its last tokens: query i of n
         has position lengths[b] - n + i.  causal: it sees the tokens up to its position, with `window` > 0 only the last `window` of
-        them (its own among them) and the first `sinks`.  A query that sees nothing gives zeros.  scale: head_dim ** -0.5 if None.
+        them (its own among them) and the first `sinks`.  A query that sees nothing gives zeros.  Lengths are cut to the table's room.  scale: head_dim ** -0.5 if None.
         longest: a bound of the lengths that the caller knows (default: the table's width); it steers how the work is cut, never
         what is computed.  out: the result's memory, which may be q's own; rows of no sequence keep what it held."""
         if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
