@@ -494,6 +494,8 @@ def test_calls_are_not_traced_away(monkeypatch):
             torch.jit.trace(call, q)
         with pytest.raises(RuntimeError, match="recorded"):
             make_fx(call)(q)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(call, pre_dispatch=True)(q)
         for transform in (lambda: torch.func.jvp(call, (q,), (q,)), lambda: torch.func.vmap(call)(q[None]), lambda: make_fx(call, tracing_mode="fake")(q)):
             with pytest.raises(Exception):
                 transform()
