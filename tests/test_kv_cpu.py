@@ -641,3 +641,13 @@ def test_rotary_refuses_keys_of_too_few_dimensions():
         for call in (r, r.apply_):
             with pytest.raises(ValueError, match="differ"):
                 call(pos, torch.zeros(4, 32), k)
+
+
+def test_a_call_of_rotary_is_one_call_to_its_hooks(launches):
+    from torch.autograd import forward_ad
+    r, pos, seen = Rotary(32), torch.arange(2), []
+    r.register_forward_hook(lambda module, args, out: seen.append(len(args)))
+    r(pos, torch.ones(2, 4, 32), torch.ones(2, 0, 32))
+    with forward_ad.dual_level():
+        r(pos, torch.ones(2, 4, 32), forward_ad.make_dual(torch.ones(2, 1, 32), torch.ones(2, 1, 32)))
+    assert seen == [3, 3]

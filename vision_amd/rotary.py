@@ -213,10 +213,10 @@ class Rotary(nn.Module):
                 return q.clone()
             if q.numel() == 0 and k.numel() == 0:
                 return q.clone(), k.clone()
-            return (self(positions, q), k.clone()) if k.numel() == 0 else (q.clone(), self(positions, k))
+            return (self.forward(positions, q), k.clone()) if k.numel() == 0 else (q.clone(), self.forward(positions, k))
         turn, tangent = _turned, has_tangent(q)
         if k is not None and has_tangent(k) != tangent:      # torch takes no result without a tangent beside one that has it
-            return self(positions, q), self(positions, k)
+            return self.forward(positions, q), self.forward(positions, k)
         if tangent or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
             turn = _RotaryFn.apply
         yq, yk = turn(positions, frequencies, self._how, q, k)
