@@ -199,15 +199,15 @@ def call(name, *args):
 
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
-_PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
-_tracing, _modes, _included = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included
+_tracing, _modes, _functions = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_before_dispatch = torch._ops.mode_stack_state_for_pre_dispatch()
 _entries = {name: getattr(lib, name) for name in SIGNATURES}
 
 
 def call_on(device, name, *args):
     """The same on the current stream of `device` (its last argument), whichever device is current.  A kernel launched from here is
     invisible to what records torch's operators, whose program would return memory that nobody writes: refused there."""
-    if _tracing() is not None or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None) or _included(_PRE_DISPATCH):
+    if _tracing() is not None or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None) or (_functions() and _before_dispatch.count()):
         raise RuntimeError(f"{name} cannot be recorded by torch.jit.trace or make_fx: call it outside of the traced function")
     index = device.index
     if index == torch.cuda.current_device():
